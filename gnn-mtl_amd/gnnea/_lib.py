@@ -73,6 +73,44 @@ class SinkhornProblem(ctypes.Structure):
     ]
 
 
+GNNEA_NORM_RMS, GNNEA_NORM_LAYER = 0, 1
+GNNEA_GATE_NONE, GNNEA_GATE_FULL, GNNEA_GATE_ROW = 0, 1, 2
+GNNEA_ADAMW_BLOCK = 256
+GNNEA_ADAMW_CTL_BYTES = 32
+GNNEA_ATTN_FWD, GNNEA_ATTN_BWD_ROWS, GNNEA_ATTN_BWD_COLS = 0, 1, 2
+
+
+def _fields(spec):
+    """[(name, type)] of "type name name ..., type name ..."."""
+    kind = {"p": _p, "i64": _i64, "i32": _i32, "f": _f32}
+    return [(name, kind[part.split()[0]]) for part in spec.split(",") for name in part.split()[1:]]
+
+
+class NormProblem(ctypes.Structure):
+    """Mirror of ``gnnea_norm`` (include/gnnea.h)."""
+
+    _fields_ = _fields(
+        "i64 n, i32 D dtype w_dtype kind gate_mode post pre sums, f eps alpha,"
+        "p x y gate scale post_w post_b pre_w pre_b, i64 ldx ldy ldg, p r h, i64 ldr ldh,"
+        "p stats dr dh, i64 lddr lddh, p dx dy dgate, i64 lddx lddy lddg,"
+        "p dscale dpost_w dpost_b dpre_w dpre_b part")
+
+
+class AdamwTensor(ctypes.Structure):
+    """Mirror of ``gnnea_adamw_tensor`` (include/gnnea.h)."""
+
+    _fields_ = _fields("p p g m v scales, i64 n index")
+
+
+class AttnProblem(ctypes.Structure):
+    """Mirror of ``gnnea_attn`` (include/gnnea.h)."""
+
+    _fields_ = _fields(
+        "p rowptr col, i32 n_rows n_cols heads kv_heads d_head dtype, f scale,"
+        "i32 limit n_items n_long, p items long_rows long_ptr q k v, i64 ldq ldk ldv, p o,"
+        "i64 ldo, p lse dout, i64 lddo, p stat dq dk dv, i64 lddq lddk lddv")
+
+
 # name -> (restype, argtypes): every symbol include/gnnea.h declares
 SIGNATURES = {
     "gnnea_abi_version": (ctypes.c_int, []),
@@ -322,6 +360,20 @@ SIGNATURES = {
                                                   _p, _p, _p, _p, _p, _i64, _p]),
     "gnnea_margin_bwd_code_bf16": (ctypes.c_int, [_i32, _i32, _i32, _p, _p, _i64, _p, _p, _i32,
                                                   _p, _p, _i32, _p, _p, _f32, _p, _i64, _p]),
+    "gnnea_norm_fwd": (ctypes.c_int, [ctypes.POINTER(NormProblem), _p]),
+    "gnnea_norm_bwd_ws_bytes": (_i64, [_i64, _i32, ctypes.c_int]),
+    "gnnea_norm_bwd": (ctypes.c_int, [ctypes.POINTER(NormProblem), _p, _i64, _p]),
+    "gnnea_adamw_norm_parts": (_i64, [_p, _i32]),
+    "gnnea_adamw_norm": (ctypes.c_int, [_p, _i32, ctypes.c_int, _p, _i64, _p]),
+    "gnnea_adamw_begin": (ctypes.c_int, [_p, _i64, _f64, _f64, _f64, _f64, _p, ctypes.c_uint32,
+                                         _p, _p, _p]),
+    "gnnea_adamw_step": (ctypes.c_int, [_p, _i32, ctypes.c_int, ctypes.c_int, _f64, _f64, _f64,
+                                        _f64, _p, _p]),
+    "gnnea_adamw_moments": (ctypes.c_int, [_p, _i32, _p]),
+    "gnnea_attn_ws_bytes": (_i64, [ctypes.POINTER(AttnProblem), ctypes.c_int]),
+    "gnnea_attn_fwd": (ctypes.c_int, [ctypes.POINTER(AttnProblem), _p, _i64, _p]),
+    "gnnea_attn_bwd_rows": (ctypes.c_int, [ctypes.POINTER(AttnProblem), _p, _i64, _p]),
+    "gnnea_attn_bwd_cols": (ctypes.c_int, [ctypes.POINTER(AttnProblem), _p, _i64, _p]),
 }
 
 _LIB = None

@@ -1,0 +1,236 @@
+"""AdamW over many tensors in few launches, moments in 32 or 8 bits (gnnea_adamw_*).
+
+The reference trains with torch.optim.Adam (run/train_ea.py:28-34); ``AdamW`` takes its place in
+the same loop (``weight_decay=0`` is Adam), with the gradients' global norm clipped in the same
+step where ``max_norm`` is given.  The step counter and the learning rate stay on the device, so a
+step can be captured into a HIP graph as it is.
+"""
+import torch
+
+from . import _lib
+from ._lib import AdamwTensor, check, ptr, stream_of
+from .ops import FEATURE_DTYPES
+
+BLOCK = _lib.GNNEA_ADAMW_BLOCK
+
+
+def _dense(t):
+    """Whether t's elements fill memory without gaps, in whatever order of dimensions."""
+    need = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != need:
+            return False
+        need *= size
+    return True
+
+
+class AdamW(torch.optim.Optimizer):
+    """m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
+    p = p (1 - lr weight_decay) - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps).
+
+    params          fp32 or bf16 tensors on one HIP device, in any number, or groups of them
+    lr              a number, or a one-element fp32 device tensor (read at every step, also by a
+                    captured graph)
+    state_bits      32, or 8: m in e4m3 and sqrt(v) in 8 bits without a sign, each with one
+                    exponent per 256 elements; sqrt(v) is rounded up or down by chance (``seed``),
+                    so that small changes are kept on average
+    max_norm        scale the gradients of all groups together down to this norm (None: no
+                    clipping).  The norm is then in ``grad_norm`` (a device tensor), and a step
+                    whose norm is not finite changes nothing; without it, such gradients reach
+                    the parameters as in torch.
+    A parameter without a gradient is left as it is.  t counts the steps of a group."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+                 state_bits=32, max_norm=None, seed=0):
+        if isinstance(lr, torch.Tensor):
+            if lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
+                raise ValueError("gnnea.AdamW: a tensor lr must be one fp32 value on the device")
+        elif not lr >= 0:
+            raise ValueError("gnnea.AdamW: lr must not be negative (got %r)" % (lr,))
+        if not eps > 0 or not weight_decay >= 0:
+            raise ValueError("gnnea.AdamW: eps must be positive and weight_decay not negative")
+        if len(betas) != 2 or not all(0 <= b < 1 for b in betas):
+            raise ValueError("gnnea.AdamW: betas must be in [0, 1) (got %r)" % (betas,))
+        if state_bits not in (8, 32):
+            raise ValueError("gnnea.AdamW: state_bits must be 8 or 32 (got %r)" % (state_bits,))
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError("gnnea.AdamW: max_norm must be positive (got %r)" % (max_norm,))
+        self.state_bits, self.max_norm = state_bits, max_norm
+        self.seed = int(seed) & 0xffffffff
+        self.grad_norm = None
+        self._index = {}  # parameter -> its number in the hash of the 8-bit rounding
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dtype not in FEATURE_DTYPES:
+                raise TypeError("gnnea.AdamW: fp32 or bf16 parameters required (got %s)" % p.dtype)
+            if p.is_sparse or not _dense(p):
+                raise ValueError("gnnea.AdamW: parameters must be dense and without gaps")
+            self._index[p] = len(self._index)
+
+    def _init_state(self, p, step):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("gnnea.AdamW: take one step before capturing (a captured first "
+                               "step would set the moments to zero at every replay)")
+        s = self.state[p]
+        s["step"] = step
+        if self.state_bits == 32:
+            s["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+            s["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+        else:
+            n = p.numel()
+            s["exp_avg"] = torch.zeros(n, dtype=torch.uint8, device=p.device)
+            s["exp_avg_rms"] = torch.zeros(n, dtype=torch.uint8, device=p.device)
+            # the exponents of m's and of sqrt(v)'s blocks (any valid one: every code is zero)
+            s["scales"] = torch.full((2, -(-n // BLOCK)), 127, dtype=torch.uint8, device=p.device)
+
+    def _tensor(self, t, p, g):
+        s = self.state[p]
+        t.p, t.g, t.m, t.n = p.data_ptr(), g, s["exp_avg"].data_ptr(), p.numel()
+        if self.state_bits == 32:
+            t.v = s["exp_avg_sq"].data_ptr()
+        else:
+            t.v, t.scales = s["exp_avg_rms"].data_ptr(), s["scales"].data_ptr()
+        t.index = self._index[p]
+
+    @staticmethod
+    def _gradient(p):
+        g = p.grad
+        if g.is_sparse or g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
+            raise ValueError("gnnea.AdamW: gradients must be dense and like their parameter")
+        if g.stride() != p.stride():  # the same order of elements as the parameter
+            g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
+        return g
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        groups, held = [], []
+        device = None
+        for group in self.param_groups:
+            ps = [p for p in group["params"] if p.grad is not None]
+            if not ps:
+                continue
+            _lib.require_device(*ps)
+            device = device or ps[0].device
+            if any(p.device != device for p in ps):
+                raise ValueError("gnnea.AdamW: parameters on more than one device")
+            steps = [self.state[p]["step"] for p in group["params"] if p in self.state]
+            step = steps[0] if steps else torch.zeros(1, dtype=torch.int64, device=device)
+            lists = {}
+            for p in ps:
+                if p not in self.state:
+                    self._init_state(p, step)
+                lists.setdefault(p.dtype, []).append(p)
+            arrays = []
+            for dtype, those in lists.items():
+                arr = (AdamwTensor * len(those))()
+                for t, p in zip(arr, those):
+                    g = self._gradient(p)
+                    held.append(g)
+                    self._tensor(t, p, g.data_ptr())
+                arrays.append((arr, len(those), _lib.GNNEA_BF16 if dtype == torch.bfloat16
+                               else _lib.GNNEA_F32))
+            groups.append((group, step, arrays))
+        if not groups:
+            return loss
+        L = _lib.lib()
+        with _lib.on_device(device):
+            stream = stream_of(device)
+            parts, n_parts = None, 0
+            if self.max_norm is not None:
+                counts = [[int(L.gnnea_adamw_norm_parts(a, c)) for a, c, _ in arrays]
+                          for _, _, arrays in groups]
+                n_parts = sum(map(sum, counts))
+                parts = torch.empty(max(n_parts, 1), dtype=torch.float64, device=device)
+                at = parts.data_ptr()
+                for (_, _, arrays), of in zip(groups, counts):
+                    for (a, c, code), m in zip(arrays, of):
+                        check(L.gnnea_adamw_norm(a, c, code, at, m, stream))
+                        at += 8 * m
+            for group, step, arrays in groups:
+                lr, (b1, b2) = group["lr"], group["betas"]
+                on_device = isinstance(lr, torch.Tensor)
+                ctl = torch.empty(_lib.GNNEA_ADAMW_CTL_BYTES // 4, dtype=torch.float32,
+                                  device=device)
+                check(L.gnnea_adamw_begin(ptr(parts), n_parts, self.max_norm or 0.0, b1, b2,
+                                          0.0 if on_device else lr,
+                                          ptr(lr) if on_device else None, self.seed, ptr(step),
+                                          ptr(ctl), stream))
+                for a, c, code in arrays:
+                    check(L.gnnea_adamw_step(a, c, code, self.state_bits, b1, b2, group["eps"],
+                                             group["weight_decay"], ptr(ctl), stream))
+                if self.max_norm is not None:
+                    self.grad_norm = ctl[4]
+        return loss
+
+    @torch.no_grad()
+    def moments(self):
+        """[(m, second)] of all parameters in order, (None, None) before their first step: with
+        32 bits the state's own exp_avg and exp_avg_sq; with 8 bits what the codes of m and of
+        sqrt(v) stand for, exactly, in bf16 tensors of the parameter's shape."""
+        ps = [p for group in self.param_groups for p in group["params"]]
+        if self.state_bits == 32:
+            return [(self.state[p]["exp_avg"], self.state[p]["exp_avg_sq"]) if p in self.state
+                    else (None, None) for p in ps]
+        out, have = [], [p for p in ps if p in self.state]
+        arr = (AdamwTensor * max(len(have), 1))()
+        at = 0
+        for p in ps:
+            if p not in self.state:
+                out.append((None, None))
+                continue
+            m, u = (torch.empty_like(p, dtype=torch.bfloat16) for _ in range(2))
+            self._tensor(arr[at], p, u.data_ptr())
+            arr[at].p = m.data_ptr()
+            at += 1
+            out.append((m, u))
+        if have:
+            with _lib.on_device(have[0].device):
+                check(_lib.lib().gnnea_adamw_moments(arr, at, stream_of(have[0].device)))
+        return out
+
+    def load_state_dict(self, state_dict):
+        """Takes the state as it is (codes stay uint8, moments of bf16 parameters stay fp32)."""
+        saved = state_dict["param_groups"]
+        if len(saved) != len(self.param_groups) or any(
+                len(a["params"]) != len(b["params"]) for a, b in zip(saved, self.param_groups)):
+            raise ValueError("gnnea.AdamW: the loaded state has other parameter groups")
+        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_rms",
+                                                                        "scales")
+        dtype = torch.float32 if self.state_bits == 32 else torch.uint8
+        new = {}
+        for old, group in zip(saved, self.param_groups):
+            ps = dict(zip(old["params"], group["params"]))
+            step = None
+            for key, p in ps.items():
+                got = state_dict["state"].get(key)
+                if not got:
+                    continue
+                if step is None:
+                    step = torch.as_tensor(got["step"]).reshape(1).to(torch.int64, copy=True).to(
+                        p.device)
+                n = p.numel()
+                shapes = dict(exp_avg=p.shape if self.state_bits == 32 else (n,),
+                              exp_avg_sq=p.shape, exp_avg_rms=(n,), scales=(2, -(-n // BLOCK)))
+                s = dict(step=step)
+                for name in names:
+                    t = got.get(name)
+                    if t is None or t.dtype != dtype or tuple(t.shape) != tuple(shapes[name]):
+                        raise ValueError("gnnea.AdamW: %s of parameter %s must be %s %s for "
+                                         "state_bits=%d" % (name, key, tuple(shapes[name]), dtype,
+                                                            self.state_bits))
+                    like = p if t.dim() == p.dim() and t.shape == p.shape and \
+                        self.state_bits == 32 else None
+                    s[name] = torch.empty_like(like, dtype=dtype) if like is not None else \
+                        torch.empty(t.shape, dtype=dtype, device=p.device)
+                    s[name].copy_(t)
+                new[p] = s
+            group.update({k: v for k, v in old.items() if k != "params"})
+        self.state.clear()
+        self.state.update(new)

@@ -844,6 +844,144 @@ int gnnea_margin_bwd_code_bf16(int32_t D, int32_t t, int32_t k, const float* m, 
                                int32_t n_long, float* scratch, const float* grad_loss,
                                float scale, void* grad, int64_t ldg, void* stream);
 
+/* ------------------------------------------------------------------------------------------ *
+ * Norms before and after a block, with its gate and residual scale (beside the HighWay layer of
+ * layers/layers.py:45-80, which has the gate and the residual without norms):
+ *   r = x + alpha * scale * sigmoid(gate) * N(y),   h = N'(r)
+ * N(y) = n post_w + post_b with n the row of y less its mean over its deviation
+ * (GNNEA_NORM_LAYER) or over its root mean square (GNNEA_NORM_RMS); post = 0: N(y) = y.  N' alike
+ * with pre_w, pre_b; pre = 0: no h.  y = NULL (then pre = 1, no gate, scale, post): h = N'(x).
+ * x, y, r, h, the full gate and their gradients: n rows of D values of `dtype` (GNNEA_F32 or
+ * GNNEA_BF16), row strides ld* >= D in elements, any alignment of an element.  scale, post_*,
+ * pre_* and the row gate (GNNEA_GATE_ROW: one vector for all rows): D values of w_dtype, NULL
+ * where absent.  1 <= D <= 8192.  Statistics and sums are fp32 or more.
+ * Backward: from dr, dh (NULL: zero) to dx, dy, dgate and the vectors' gradients (NULL: not
+ * wanted); `stats` is the forward's (n x 4 floats, 16-B aligned).  Deterministic.
+ * ------------------------------------------------------------------------------------------ */
+#define GNNEA_NORM_RMS 0
+#define GNNEA_NORM_LAYER 1
+#define GNNEA_GATE_NONE 0
+#define GNNEA_GATE_FULL 1
+#define GNNEA_GATE_ROW 2
+
+typedef struct gnnea_norm {
+  int64_t n;
+  int32_t D;
+  int32_t dtype, w_dtype; /* GNNEA_F32 / GNNEA_BF16; fp32 features take fp32 vectors */
+  int32_t kind, gate_mode;
+  int32_t post, pre;
+  int32_t sums;           /* set by the library */
+  float eps, alpha;
+  const void *x, *y, *gate, *scale, *post_w, *post_b, *pre_w, *pre_b;
+  int64_t ldx, ldy, ldg;
+  void *r, *h;            /* forward */
+  int64_t ldr, ldh;
+  float* stats;           /* forward: written unless NULL; backward: read */
+  const void *dr, *dh;    /* backward */
+  int64_t lddr, lddh;
+  void *dx, *dy, *dgate;
+  int64_t lddx, lddy, lddg;
+  void *dscale, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+  float* part;            /* set by the library */
+} gnnea_norm;
+
+int gnnea_norm_fwd(const gnnea_norm* a, void* stream);
+int64_t gnnea_norm_bwd_ws_bytes(int64_t n, int32_t D, int dtype);
+int gnnea_norm_bwd(const gnnea_norm* a, void* ws /* 16-B aligned */, int64_t ws_bytes,
+                   void* stream);
+
+/* ------------------------------------------------------------------------------------------ *
+ * AdamW over many tensors (the optimizer step of run/train_ea.py:64, there torch's Adam):
+ *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  t = step + 1
+ *   p = p (1 - lr wd) - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+ * with g first multiplied by min(1, max_norm / (norm + 1e-6)), norm the 2-norm of all gradients.
+ * Moments in 32 bits (m, v: n floats) or in 8 (m, v: n codes, scales: 2 x ceil(n / 256) bytes,
+ * the exponents of m's blocks of 256 and then of v's):
+ *   m: e4m3, nearest even, times 2^(scales[0][b] - 127)
+ *   v: its root u, unsigned; code 0 is 0, else (1 + (c % 16) / 16) 2^(c / 16 - 15) times
+ *      2^(scales[1][b] - 127); rounded up or down with the odds of its place between two codes,
+ *      by a hash of (seed, t, tensor, element)
+ * The update uses the moments before they are rounded.  p and g have one type (GNNEA_F32 or
+ * GNNEA_BF16) and any alignment; `tensors` is host memory, read before the call returns.
+ *   gnnea_adamw_norm   sums of squares of the gradients, gnnea_adamw_norm_parts(...) doubles
+ *   gnnea_adamw_begin  one launch before the updates of a step: folds `parts` sums (0: no clipping),
+ *                      takes t = step + 1 and writes ctl (GNNEA_ADAMW_CTL_BYTES, 8-B aligned):
+ *                      floats {factor of g, 1 / (1 - b1^t), 1 / sqrt(1 - b2^t), lr, norm}, then two
+ *                      words {hash key, 1 = leave everything as it is}; a norm that is not finite
+ *                      sets the latter and leaves step as it is, unless max_norm <= 0
+ *   gnnea_adamw_step   the update of `count` tensors
+ *   gnnea_adamw_moments  what 8-bit codes stand for, in bf16 (exact): m to p, u to g
+ * ------------------------------------------------------------------------------------------ */
+#define GNNEA_ADAMW_BLOCK 256
+#define GNNEA_ADAMW_CTL_BYTES 32
+
+typedef struct gnnea_adamw_tensor {
+  void* p;
+  const void* g;
+  void *m, *v;
+  uint8_t* scales; /* 8-bit moments only */
+  int64_t n;
+  int64_t index;   /* the tensor's number in the hash */
+} gnnea_adamw_tensor;
+
+int64_t gnnea_adamw_norm_parts(const gnnea_adamw_tensor* tensors, int32_t count);
+int gnnea_adamw_norm(const gnnea_adamw_tensor* tensors, int32_t count, int dtype, double* parts,
+                     int64_t n_parts, void* stream);
+int gnnea_adamw_begin(const double* parts, int64_t n_parts, double max_norm, double beta1,
+                      double beta2, double lr, const float* lr_dev /* nullable: wins */,
+                      uint32_t seed, int64_t* step, void* ctl, void* stream);
+int gnnea_adamw_step(const gnnea_adamw_tensor* tensors, int32_t count, int dtype, int state_bits,
+                     double beta1, double beta2, double eps, double weight_decay,
+                     const void* ctl, void* stream);
+int gnnea_adamw_moments(const gnnea_adamw_tensor* tensors, int32_t count, void* stream);
+
+/* ------------------------------------------------------------------------------------------ *
+ * Dot-product attention over the stored entries of a sparse matrix (beside the additive scores of
+ * layers/att_layers.py:29-61): for row i and head h, with key/value head j = h / (heads / kv_heads),
+ *   o_i = sum_c p_ic v_c,   p_ic = softmax over the row's entries c of (scale q_i . k_c)
+ * q, o: n_rows x heads d_head; k, v: n_cols x kv_heads d_head (type GNNEA_F32 or GNNEA_BF16, row
+ * strides in elements, any alignment of an element); lse: n_rows x heads floats, the log of the
+ * row's sum of exponentials; a row without entries gives o = 0 and lse = -inf.  k and v of columns
+ * that no row has stored are never read.  heads % kv_heads == 0, d_head <= 256.  The matrix's
+ * values are not used.
+ * Backward, the probabilities recomputed as p = exp(scale q.k - lse), dp = do . v:
+ *   _bwd_rows  dq_i = scale (sum p dp k - delta sum p k), delta_i = sum p dp, over the matrix's
+ *              rows; writes stat: n_rows x heads x {lse in powers of two, delta} floats
+ *   _bwd_cols  dk, dv (summed over the heads that share a key/value head) over the transposed
+ *              matrix's rows; reads stat
+ * Rows of dq, dk, dv without entries are written with zeros.  Sums are fp32 in a fixed order.
+ * Rows of more than `limit` entries (0: none) are left to pieces: items {row, begin, end, slot}
+ * (int32 x 4; slots 0 .. n_items - 1) and, joined in order, long_rows with their slots
+ * long_ptr[w] .. long_ptr[w + 1] - 1.  They depend on rowptr alone (built once per matrix).
+ * ------------------------------------------------------------------------------------------ */
+typedef struct gnnea_attn {
+  const int32_t *rowptr, *col;   /* the CSR; _bwd_cols: the transposed one */
+  int32_t n_rows, n_cols;        /* of this CSR */
+  int32_t heads, kv_heads, d_head;
+  int32_t dtype;
+  float scale;
+  int32_t limit, n_items, n_long;
+  const int32_t *items, *long_rows, *long_ptr;
+  const void *q, *k, *v;
+  int64_t ldq, ldk, ldv;
+  void* o;                       /* forward */
+  int64_t ldo;
+  float* lse;                    /* forward: written unless NULL; _bwd_rows: read */
+  const void* dout;              /* backward */
+  int64_t lddo;
+  float* stat;                   /* 8-B aligned */
+  void *dq, *dk, *dv;
+  int64_t lddq, lddk, lddv;
+} gnnea_attn;
+
+#define GNNEA_ATTN_FWD 0
+#define GNNEA_ATTN_BWD_ROWS 1
+#define GNNEA_ATTN_BWD_COLS 2
+int64_t gnnea_attn_ws_bytes(const gnnea_attn* a, int pass /* GNNEA_ATTN_* */);
+int gnnea_attn_fwd(const gnnea_attn* a, void* ws, int64_t ws_bytes, void* stream);
+int gnnea_attn_bwd_rows(const gnnea_attn* a, void* ws, int64_t ws_bytes, void* stream);
+int gnnea_attn_bwd_cols(const gnnea_attn* a, void* ws, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
