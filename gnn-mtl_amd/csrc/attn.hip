@@ -24,50 +24,58 @@
 namespace gnnea {
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLn2 = 0.69314718055994530942f;
 
-struct AttnPlan { int lph, nch, hpw, units_y; };
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-// the 16-B chunks of a head that a lane holds
-template <typename T, int LPH, int NCH> struct Lane {
+struct AttnPlan { int lph, nch, hpw, units_y; bool full; };
+
+// The 16-B chunks of a head that a lane holds: NCH of them, LPH lanes apart.  FULL: d_head is
+// LPH NCH V.  Otherwise a head's last chunk is moved back so that it ends with the head, and holds
+// values of the lane before first; lanes past it hold none.
+template <typename T, int LPH, int NCH, bool FULL> struct Lane {
   static constexpr int V = RowChunk<T>::V;
   int dh, l;
-  // first element of chunk c: the last chunk of a head is moved back so that it ends with the head
+  __device__ __forceinline__ int first(int c) const { return (c * LPH + l) * V; }
   __device__ __forceinline__ int at(int c) const {
-    const int e = (c * LPH + l) * V;
-    return dh >= V && e > dh - V ? dh - V : e;
+    const int e = first(c);
+    if (FULL || c < NCH - 1) return e;
+    return dh >= V ? (e > dh - V ? dh - V : e) : 0;
   }
-  __device__ __forceinline__ bool has(int c) const { return (c * LPH + l) * V < dh; }
-  // whether element k of chunk c is this lane's own (not one that the lane before also holds)
+  __device__ __forceinline__ bool has(int c) const { return FULL || c < NCH - 1 || first(c) < dh; }
+  // whether value k of chunk c is the lane's own
   __device__ __forceinline__ bool own(int c, int k) const {
+    if (FULL || c < NCH - 1) return true;
     const int e = at(c) + k;
-    return e >= (c * LPH + l) * V && e < dh;
+    return has(c) && e >= first(c) && e < dh;
   }
-  __device__ __forceinline__ uint4 raw(const T* p, int c, bool ok) const {
-    uint4 r = make_uint4(0, 0, 0, 0);
-    if (ok && has(c)) {
-      if (dh >= V) {
-        r = load16<T>(p + at(c));
-      } else {  // heads narrower than 16 B: element by element
-        uint32_t w[4] = {0, 0, 0, 0};
+  // chunk c of the head at p; 0 for lanes without one
+  __device__ __forceinline__ uint4 raw(const T* p, int c) const {
+    if constexpr (FULL) return load16<T>(p + first(c));
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (has(c)) {
+      if (dh >= V) return load16<T>(p + at(c));
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (k < dh) {
-            if constexpr (V == 4) w[k] = __builtin_bit_cast(uint32_t, (float)to_f32<T>(p[k]));
-            else w[k / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[k]) << (16 * (k & 1));
-          }
-        r = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+      for (int k = 0; k < V; ++k)  // heads narrower than 16 B: element by element
+        if (k < dh) {
+          if constexpr (V == 4) w[k] = __builtin_bit_cast(uint32_t, (float)to_f32<T>(p[k]));
+          else w[k / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[k]) << (16 * (k & 1));
+        }
     }
-    return r;
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // the lane's own elements, times s; 0 elsewhere
-  __device__ __forceinline__ void load_own(const T* p, bool ok, float s, float (&f)[NCH][V]) const {
+  // r with 0 in the places that are not the lane's own (ok: in all)
+  __device__ __forceinline__ uint4 mask(const uint4& r, int c, bool ok) const {
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (!ok || !own(c, k)) w[k * 4 / V] &= V == 4 ? 0u : (k & 1) ? 0xffffu : 0xffff0000u;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ void load_own(const T* p, bool ok, uint4 (&f)[NCH]) const {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      unpack16(raw(p, c, ok), f[c]);
-#pragma unroll
-      for (int k = 0; k < V; ++k) f[c][k] = own(c, k) ? f[c][k] * s : 0.f;
+      f[c] = make_uint4(0, 0, 0, 0);
+      if (ok) f[c] = FULL || c < NCH - 1 ? raw(p, c) : mask(raw(p, c), c, true);
     }
   }
   template <typename O>
@@ -75,13 +83,12 @@ template <typename T, int LPH, int NCH> struct Lane {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       if (!has(c)) continue;
-      const int e = (c * LPH + l) * V;
       float g[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) g[k] = f[c][k] * s;
       if constexpr (sizeof(O) == sizeof(T)) {
-        if (e + V <= dh) {
-          store_chunk<T, V>((T*)p + e, V, g);
+        if (FULL || first(c) + V <= dh) {
+          store_chunk<T, V>((T*)p + first(c), V, g);
           continue;
         }
       }
@@ -93,22 +100,6 @@ template <typename T, int LPH, int NCH> struct Lane {
   }
 };
 
-template <int V>
-__device__ __forceinline__ float dot(const float (&a)[V], const uint4& raw, float s) {
-  float b[V];
-  unpack16(raw, b);
-#pragma unroll
-  for (int k = 0; k < V; ++k) s = fmaf(a[k], b[k], s);
-  return s;
-}
-template <int V>
-__device__ __forceinline__ void axpy(float a, const uint4& raw, float (&y)[V]) {
-  float b[V];
-  unpack16(raw, b);
-#pragma unroll
-  for (int k = 0; k < V; ++k) y[k] = fmaf(a, b[k], y[k]);
-}
-
 // the sum over a group's LPH lanes, in all of them
 template <int LPH>
 __device__ __forceinline__ float group_sum(float v) {
@@ -119,84 +110,203 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+// the value of lane ^ w (w a power of two; 32, 16 and 8 without LDS)
+__device__ __forceinline__ float lane_xor(float v, int w) {
+  const uint32_t x = __builtin_bit_cast(uint32_t, v);
+  if (w == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __builtin_bit_cast(float, lane_id() < 32 ? r[1] : r[0]);
+  }
+  if (w == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return __builtin_bit_cast(float, (lane_id() & 16) == 0 ? r[1] : r[0]);
+  }
+  if (w == 8) return mov_dpp_f32<0x128>(v);  // row_ror:8
+  return __shfl_xor(v, w, 64);
+}
+
+// The products of a head's fp32 values, or of its bf16 pairs (each exact), summed over the group.
+template <int V, int LPH, int NCH>
+__device__ __forceinline__ float head_dot(const uint4 (&a)[NCH], const uint4 (&b)[NCH]) {
+  float s = 0.f;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const uint32_t x[4] = {a[c].x, a[c].y, a[c].z, a[c].w}, y[4] = {b[c].x, b[c].y, b[c].z, b[c].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (V == 4)
+        s = fmaf(__builtin_bit_cast(float, x[k]), __builtin_bit_cast(float, y[k]), s);
+      else
+        s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x[k]),
+                                            __builtin_bit_cast(bf16x2, y[k]), s, false);
+    }
+  }
+  return group_sum<LPH>(s);
+}
+template <int V>
+__device__ __forceinline__ void axpy(float a, const uint4& raw, float (&y)[V]) {
+  float b[V];
+  unpack16(raw, b);
+#pragma unroll
+  for (int k = 0; k < V; ++k) y[k] = fmaf(a, b[k], y[k]);
+}
+// + 0 times the values: NaN where one of them is not finite
+template <int NCH, int V>
+__device__ __forceinline__ float zero_of(const float (&f)[NCH][V], float s) {
+#pragma unroll
+  for (int c = 0; c < NCH; ++c)
+#pragma unroll
+    for (int k = 0; k < V; ++k) s = fmaf(f[c][k], 0.f, s);
+  return s;
+}
+template <int NCH, int V>
+__device__ __forceinline__ void clear(float (&f)[NCH][V]) {
+#pragma unroll
+  for (int c = 0; c < NCH; ++c)
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[c][k] = 0.f;
+}
+
 struct AttnUnit { int row, beg, end, slot; };
 
-// The wave's row, or piece of a row (slot >= 0).  False: nothing to do.
-__device__ __forceinline__ bool attn_unit(const gnnea_attn& a, bool pieces, AttnUnit& u) {
-  const int id = blockIdx.x * 4 + wave_id();
-  if (pieces) {
-    if (id >= a.n_items) return false;
+// The wave's piece of a long row (these come first: they run longest), or its row (slot < 0).
+// False: nothing to do.
+__device__ __forceinline__ bool attn_unit(const gnnea_attn& a, AttnUnit& u) {
+  int id = blockIdx.x * 4 + wave_id();
+  if (id < a.n_items) {
     const int4 it = ((const int4*)a.items)[id];
     u.row = it.x; u.beg = it.y; u.end = it.z; u.slot = it.w;
     return true;
   }
+  id -= a.n_items;
   if (id >= a.n_rows) return false;
   u.row = id; u.beg = a.rowptr[id]; u.end = a.rowptr[id + 1]; u.slot = -1;
   return a.limit == 0 || u.end - u.beg <= a.limit;
 }
 
-template <int NCH> struct Steps { static constexpr int U = NCH == 1 ? 4 : 2; };
+// Entries that a group loads before it computes any.  More in flight per wave cost registers, and
+// with them waves: at 290k entries, 4 heads of 75 fp32 (three chunks) the row pass takes 107, 115
+// and 144 us with 1, 2 and 3, the column pass 119, 128 and 163; at 3.3M entries, 8 heads of 32 bf16
+// (one chunk) the three passes take 1053, 1014 and 1164 us with 1, 2 and 4.
+template <int NCH> struct Steps { static constexpr int U = NCH <= 2 ? 2 : 1; };
 
-template <typename T, int LPH, int NCH>
-__global__ __launch_bounds__(256) void k_attn_fwd(const gnnea_attn a, int hpw, bool pieces,
+// The next 64 columns of the unit's entries, one per lane, read while the current ones are used.
+// Lanes past the end repeat the last entry: what is read for them is the row's own, and weighs 0.
+struct ColBatch {
+  int now, next, left;
+  __device__ __forceinline__ ColBatch(const int32_t* col, int beg, int end) {
+    next = now = left = 0;
+    if (beg < end) next = col[min(beg + lane_id(), end - 1)];
+  }
+  __device__ __forceinline__ void step(const int32_t* col, int at, int end) {
+    now = next;
+    left = min(end - at, 64);
+    if (at + 64 < end) next = col[min(at + 64 + lane_id(), end - 1)];
+  }
+};
+
+// The row offsets (in elements) of a lane's column in a table, formed once per 64 entries and
+// handed to the group that reads the entry; the high words only where a table has them.
+struct RowOffset {
+  uint32_t lo, hi;
+  bool wide;
+  __device__ __forceinline__ RowOffset(int32_t rows, int64_t ld) : lo(0), hi(0) {
+    wide = (int64_t)rows * ld > 0xffffffffll;
+  }
+  __device__ __forceinline__ void set(int col, int64_t ld) {
+    const uint64_t o = (uint64_t)(uint32_t)col * (uint64_t)ld;
+    lo = (uint32_t)o;
+    hi = (uint32_t)(o >> 32);
+  }
+  __device__ __forceinline__ uint64_t of(int lane) const {
+    uint64_t o = (uint32_t)__shfl((int)lo, lane, 64);
+    if (wide) o |= (uint64_t)(uint32_t)__shfl((int)hi, lane, 64) << 32;
+    return o;
+  }
+};
+
+// A lane's row of scores: keys and values of U entries at a time.  `care`: a second run of a unit
+// whose sums came out not finite, with 0 in every place that is not an entry's own (0 times an
+// infinity read for nothing is not 0).
+template <typename T, int LPH, int NCH, bool FULL>
+__global__ __launch_bounds__(256) void k_attn_fwd(const gnnea_attn a, int hpw,
                                                   float* __restrict__ ws) {
   constexpr int V = RowChunk<T>::V, G = 64 / LPH, U = Steps<NCH>::U;
   AttnUnit u;
-  if (!attn_unit(a, pieces, u)) return;
+  if (!attn_unit(a, u)) return;
   const int lane = lane_id(), grp = lane / LPH, dh = a.d_head;
-  const Lane<T, LPH, NCH> L{dh, lane % LPH};
+  const Lane<T, LPH, NCH, FULL> L{dh, lane % LPH};
   const int head = blockIdx.y * hpw + grp % hpw, slot = grp / hpw, eps = G / hpw;
   const bool on = head < a.heads;
   const int64_t kvo = (int64_t)(on ? head / (a.heads / a.kv_heads) : 0) * dh;
   const T* K = (const T*)a.k + kvo;
   const T* Vp = (const T*)a.v + kvo;
-  float q[NCH][V], o[NCH][V], m = -INFINITY, sum = 0.f;
-  L.load_own((const T*)a.q + u.row * a.ldq + (int64_t)head * dh, on, a.scale * kLog2e, q);
+  const float factor = a.scale * kLog2e;
+  uint4 q[NCH];
+  float o[NCH][V], m, sum;
+  for (bool care = false;; care = true) {
+    ColBatch cb(a.col, u.beg, u.end);
+    RowOffset off(a.n_cols, a.ldk);
+    L.load_own((const T*)a.q + u.row * a.ldq + (int64_t)head * dh, on, q);
+    m = -INFINITY;
+    sum = 0.f;
+    clear(o);
+    for (int at = u.beg; at < u.end; at += 64) {
+      cb.step(a.col, at, u.end);
+      off.set(cb.now, a.ldk);
+      for (int b = 0; b < cb.left; b += eps * U) {
+        uint4 rk[U][NCH], rv[U][NCH];
+        bool ok[U];
 #pragma unroll
-  for (int c = 0; c < NCH; ++c)
+        for (int s = 0; s < U; ++s) {
+          const int e = b + s * eps + slot;
+          ok[s] = on && e < cb.left;
+          const uint64_t j = off.of(min(e, 63));
 #pragma unroll
-    for (int k = 0; k < V; ++k) o[c][k] = 0.f;
-  for (int b = u.beg; b < u.end; b += eps * U) {
-    uint4 rk[U][NCH], rv[U][NCH];
-    bool ok[U];
+          for (int c = 0; c < NCH; ++c) rk[s][c] = L.raw(K + j, c);
 #pragma unroll
-    for (int s = 0; s < U; ++s) {
-      const int e = b + s * eps + slot;
-      ok[s] = on && e < u.end;
-      const int64_t j = ok[s] ? a.col[e] : 0;
+          for (int c = 0; c < NCH; ++c) rv[s][c] = L.raw(Vp + j, c);
+        }
+        if (care) {
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) rk[s][c] = L.raw(K + j * a.ldk, c, ok[s]);
+          for (int s = 0; s < U; ++s)
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) rv[s][c] = L.raw(Vp + j * a.ldv, c, ok[s]);
+            for (int c = 0; c < NCH; ++c) {
+              rk[s][c] = L.mask(rk[s][c], c, ok[s]);
+              rv[s][c] = L.mask(rv[s][c], c, ok[s]);
+            }
+        }
+        float x[U], top = m;
+#pragma unroll
+        for (int s = 0; s < U; ++s) {
+          const float d = head_dot<V, LPH>(q, rk[s]) * factor;
+          x[s] = ok[s] ? d : -INFINITY;
+          top = x[s] > top || x[s] != x[s] ? x[s] : top;
+        }
+        const float ref = top == -INFINITY ? 0.f : top;  // only -inf so far: all weights are 0
+        if (at + b > u.beg) {                            // (o and sum are 0 before the first)
+          const float keep = __builtin_amdgcn_exp2f(m - ref);
+          sum *= keep;
+#pragma unroll
+          for (int c = 0; c < NCH; ++c)
+#pragma unroll
+            for (int k = 0; k < V; ++k) o[c][k] *= keep;
+        }
+        m = top;
+#pragma unroll
+        for (int s = 0; s < U; ++s) {
+          const float p = __builtin_amdgcn_exp2f(x[s] - ref);
+          sum += p;
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) axpy<V>(p, rv[s][c], o[c]);
+        }
+      }
     }
-    float x[U], top = m;
-#pragma unroll
-    for (int s = 0; s < U; ++s) {
-      float d = 0.f;
-#pragma unroll
-      for (int c = 0; c < NCH; ++c) d = dot<V>(q[c], rk[s][c], d);
-      d = group_sum<LPH>(d);
-      x[s] = ok[s] ? d : -INFINITY;
-      top = x[s] > top || x[s] != x[s] ? x[s] : top;
-    }
-    const float ref = top == -INFINITY ? 0.f : top;  // nothing but -inf so far: all weights 0
-    const float keep = __builtin_amdgcn_exp2f(m - ref);
-    m = top;
-    sum *= keep;
-#pragma unroll
-    for (int c = 0; c < NCH; ++c)
-#pragma unroll
-      for (int k = 0; k < V; ++k) o[c][k] *= keep;
-#pragma unroll
-    for (int s = 0; s < U; ++s) {
-      const float p = __builtin_amdgcn_exp2f(x[s] - ref);
-      sum += p;
-#pragma unroll
-      for (int c = 0; c < NCH; ++c) axpy<V>(p, rv[s][c], o[c]);
-    }
+    const float z = on ? zero_of(o, sum * 0.f) : 0.f;
+    if (care || !__any(z != z)) break;
   }
   for (int w = LPH * hpw; w < 64; w <<= 1) {  // the groups of one head
-    const float mo = __shfl_xor(m, w, 64), so = __shfl_xor(sum, w, 64);
+    const float mo = lane_xor(m, w), so = lane_xor(sum, w);
     const float top = mo > m || mo != mo ? mo : m;
     const float ref = top == -INFINITY ? 0.f : top;
     const float ka = __builtin_amdgcn_exp2f(m - ref), kb = __builtin_amdgcn_exp2f(mo - ref);
@@ -205,10 +315,10 @@ __global__ __launch_bounds__(256) void k_attn_fwd(const gnnea_attn a, int hpw, b
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
-      for (int k = 0; k < V; ++k) o[c][k] = o[c][k] * ka + __shfl_xor(o[c][k], w, 64) * kb;
+      for (int k = 0; k < V; ++k) o[c][k] = o[c][k] * ka + lane_xor(o[c][k], w) * kb;
   }
   if (slot != 0 || !on) return;
-  if (pieces) {
+  if (u.slot >= 0) {
     float* part = ws + ((int64_t)u.slot * a.heads + head) * (dh + 2);
     if (L.l == 0) part[0] = m, part[1] = sum;
     L.store(part + 2, o, 1.f);
@@ -216,76 +326,89 @@ __global__ __launch_bounds__(256) void k_attn_fwd(const gnnea_attn a, int hpw, b
   }
   L.store((T*)a.o + u.row * a.ldo + (int64_t)head * dh, o, sum == 0.f ? 0.f : 1.f / sum);
   if (a.lse && L.l == 0)
-    a.lse[(int64_t)u.row * a.heads + head] = sum == 0.f ? -INFINITY : fmaf(m, kLn2, logf(sum));
+    a.lse[(int64_t)u.row * a.heads + head] = sum == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(sum);
 }
 
-template <typename T, int LPH, int NCH>
-__global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, int hpw, bool pieces,
+template <typename T, int LPH, int NCH, bool FULL>
+__global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, int hpw,
                                                    float* __restrict__ ws) {
   constexpr int V = RowChunk<T>::V, G = 64 / LPH, U = Steps<NCH>::U;
   AttnUnit u;
-  if (!attn_unit(a, pieces, u)) return;
+  if (!attn_unit(a, u)) return;
   const int lane = lane_id(), grp = lane / LPH, dh = a.d_head;
-  const Lane<T, LPH, NCH> L{dh, lane % LPH};
+  const Lane<T, LPH, NCH, FULL> L{dh, lane % LPH};
   const int head = blockIdx.y * hpw + grp % hpw, slot = grp / hpw, eps = G / hpw;
   const bool on = head < a.heads;
   const int64_t kvo = (int64_t)(on ? head / (a.heads / a.kv_heads) : 0) * dh;
   const T* K = (const T*)a.k + kvo;
   const T* Vp = (const T*)a.v + kvo;
-  float q[NCH][V], d[NCH][V], A[NCH][V], B[NCH][V], delta = 0.f;
-  L.load_own((const T*)a.q + u.row * a.ldq + (int64_t)head * dh, on, a.scale * kLog2e, q);
-  L.load_own((const T*)a.dout + u.row * a.lddo + (int64_t)head * dh, on, 1.f, d);
-  const float lse = on ? a.lse[(int64_t)u.row * a.heads + head] * kLog2e : 0.f;
+  const float factor = a.scale * kLog2e;
+  const float lse = on ? a.lse[(int64_t)u.row * a.heads + head] : -INFINITY;
+  uint4 q[NCH], d[NCH];
+  float A[NCH][V], B[NCH][V], delta;
+  for (bool care = false;; care = true) {
+    ColBatch cb(a.col, u.beg, u.end);
+    RowOffset off(a.n_cols, a.ldk);
+    L.load_own((const T*)a.q + u.row * a.ldq + (int64_t)head * dh, on, q);
+    L.load_own((const T*)a.dout + u.row * a.lddo + (int64_t)head * dh, on, d);
+    delta = 0.f;
+    clear(A);
+    clear(B);
+    for (int at = u.beg; at < u.end; at += 64) {
+      cb.step(a.col, at, u.end);
+      off.set(cb.now, a.ldk);
+      for (int b = 0; b < cb.left; b += eps * U) {
+        uint4 rk[U][NCH], rv[U][NCH];
+        bool ok[U];
 #pragma unroll
-  for (int c = 0; c < NCH; ++c)
+        for (int s = 0; s < U; ++s) {
+          const int e = b + s * eps + slot;
+          // a row whose scores are all -inf has no weights (lse = -inf), like one without entries
+          ok[s] = lse != -INFINITY && e < cb.left;
+          const uint64_t j = off.of(min(e, 63));
 #pragma unroll
-    for (int k = 0; k < V; ++k) A[c][k] = B[c][k] = 0.f;
-  for (int b = u.beg; b < u.end; b += eps * U) {
-    uint4 rk[U][NCH], rv[U][NCH];
-    bool ok[U];
+          for (int c = 0; c < NCH; ++c) rk[s][c] = L.raw(K + j, c);
 #pragma unroll
-    for (int s = 0; s < U; ++s) {
-      const int e = b + s * eps + slot;
-      ok[s] = on && e < u.end;
-      const int64_t j = ok[s] ? a.col[e] : 0;
+          for (int c = 0; c < NCH; ++c) rv[s][c] = L.raw(Vp + j, c);
+        }
+        if (care) {
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) rk[s][c] = L.raw(K + j * a.ldk, c, ok[s]);
+          for (int s = 0; s < U; ++s)
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) rv[s][c] = L.raw(Vp + j * a.ldv, c, ok[s]);
-    }
+            for (int c = 0; c < NCH; ++c) {
+              rk[s][c] = L.mask(rk[s][c], c, ok[s]);
+              rv[s][c] = L.mask(rv[s][c], c, ok[s]);
+            }
+        }
 #pragma unroll
-    for (int s = 0; s < U; ++s) {
-      float x = 0.f, y = 0.f;
+        for (int s = 0; s < U; ++s) {
+          const float x = head_dot<V, LPH>(q, rk[s]), y = head_dot<V, LPH>(d, rv[s]);
+          const float p = ok[s] ? __builtin_amdgcn_exp2f(fmaf(x, factor, -lse)) : 0.f;
+          const float pd = p * y;
+          delta += pd;
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        x = dot<V>(q[c], rk[s][c], x);
-        y = dot<V>(d[c], rv[s][c], y);
+          for (int c = 0; c < NCH; ++c) {
+            axpy<V>(pd, rk[s][c], A[c]);
+            axpy<V>(p, rk[s][c], B[c]);
+          }
+        }
       }
-      x = group_sum<LPH>(x);
-      y = group_sum<LPH>(y);
-      // a row whose scores are all -inf has no weights (lse = -inf), like one without entries
-      const float p = ok[s] && lse != -INFINITY ? __builtin_amdgcn_exp2f(x - lse) : 0.f;
-      const float pd = ok[s] ? p * y : 0.f;
-      delta += pd;
-#pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        axpy<V>(pd, rk[s][c], A[c]);
-        axpy<V>(p, rk[s][c], B[c]);
-      }
     }
+    const float z = on ? zero_of(A, zero_of(B, delta * 0.f)) : 0.f;
+    if (care || !__any(z != z)) break;
   }
   for (int w = LPH * hpw; w < 64; w <<= 1) {
-    delta += __shfl_xor(delta, w, 64);
+    delta += lane_xor(delta, w);
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        A[c][k] += __shfl_xor(A[c][k], w, 64);
-        B[c][k] += __shfl_xor(B[c][k], w, 64);
+        A[c][k] += lane_xor(A[c][k], w);
+        B[c][k] += lane_xor(B[c][k], w);
       }
   }
   if (slot != 0 || !on) return;
-  if (pieces) {
+  if (u.slot >= 0) {
     float* part = ws + ((int64_t)u.slot * a.heads + head) * (2 * dh + 1);
     if (L.l == 0) part[0] = delta;
     L.store(part + 1, A, 1.f);
@@ -303,74 +426,88 @@ __global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, int hpw, 
 
 // Columns: a row of the transposed matrix per wave; groups take key/value heads, then (entry,
 // query head of the group) pairs.
-template <typename T, int LPH, int NCH>
-__global__ __launch_bounds__(256) void k_attn_cols(const gnnea_attn a, int hpw, bool pieces,
+template <typename T, int LPH, int NCH, bool FULL>
+__global__ __launch_bounds__(256) void k_attn_cols(const gnnea_attn a, int hpw,
                                                    float* __restrict__ ws) {
   constexpr int V = RowChunk<T>::V, G = 64 / LPH, U = Steps<NCH>::U;
   AttnUnit u;
-  if (!attn_unit(a, pieces, u)) return;
+  if (!attn_unit(a, u)) return;
   const int lane = lane_id(), grp = lane / LPH, dh = a.d_head;
-  const Lane<T, LPH, NCH> L{dh, lane % LPH};
+  const Lane<T, LPH, NCH, FULL> L{dh, lane % LPH};
   const int kvh = blockIdx.y * hpw + grp % hpw, slot = grp / hpw, pps = G / hpw;
   const bool on = kvh < a.kv_heads;
   const int share = a.heads / a.kv_heads;
-  float kf[NCH][V], vf[NCH][V], dk[NCH][V], dv[NCH][V];
-  L.load_own((const T*)a.k + u.row * a.ldk + (int64_t)kvh * dh, on, a.scale * kLog2e, kf);
-  L.load_own((const T*)a.v + u.row * a.ldv + (int64_t)kvh * dh, on, 1.f, vf);
+  const float factor = a.scale * kLog2e;
+  uint4 kf[NCH], vf[NCH];
+  float dk[NCH][V], dv[NCH][V];
+  for (bool care = false;; care = true) {
+    ColBatch cb(a.col, u.beg, u.end);
+    RowOffset offq(a.n_cols, a.ldq), offd(a.n_cols, a.lddo);
+    L.load_own((const T*)a.k + u.row * a.ldk + (int64_t)kvh * dh, on, kf);
+    L.load_own((const T*)a.v + u.row * a.ldv + (int64_t)kvh * dh, on, vf);
+    clear(dk);
+    clear(dv);
+    for (int at = u.beg; at < u.end; at += 64) {
+      cb.step(a.col, at, u.end);
+      offq.set(cb.now, a.ldq);
+      offd.set(cb.now, a.lddo);
+      const int pairs = cb.left * share;  // share <= heads <= 65535: fits
+      for (int b = 0; b < pairs; b += pps * U) {
+        uint4 rq[U][NCH], rd[U][NCH];
+        float2 st[U];
+        bool ok[U];
 #pragma unroll
-  for (int c = 0; c < NCH; ++c)
+        for (int s = 0; s < U; ++s) {
+          const int t = b + s * pps + slot, f = min(t, pairs - 1);
+          ok[s] = on && t < pairs;
+          const int e = share == 1 ? f : (int)((uint32_t)f / (uint32_t)share);
+          const int h = (on ? kvh : 0) * share + f - e * share;
+          const uint64_t i = (uint32_t)__shfl(cb.now, e, 64);
+          st[s] = *(const float2*)(a.stat + 2 * (i * a.heads + h));
+          const T* Q = (const T*)a.q + (offq.of(e) + h * dh);
+          const T* Dp = (const T*)a.dout + (offd.of(e) + h * dh);
 #pragma unroll
-    for (int k = 0; k < V; ++k) dk[c][k] = dv[c][k] = 0.f;
-  const int64_t pairs = (int64_t)(u.end - u.beg) * share;
-  for (int64_t b = 0; b < pairs; b += pps * U) {
-    uint4 rq[U][NCH], rd[U][NCH];
-    float2 st[U];
-    bool ok[U];
+          for (int c = 0; c < NCH; ++c) rq[s][c] = L.raw(Q, c);
 #pragma unroll
-    for (int s = 0; s < U; ++s) {
-      const int64_t t = b + s * pps + slot;
-      ok[s] = on && t < pairs;
-      const uint32_t e = share == 1 ? (uint32_t)t : (uint32_t)((uint64_t)t / (uint32_t)share);
-      const int h = kvh * share + (int)(t - (int64_t)e * share);
-      const int64_t i = ok[s] ? a.col[u.beg + (int)e] : 0;
-      st[s] = ok[s] ? *(const float2*)(a.stat + 2 * (i * a.heads + h)) : make_float2(0.f, 0.f);
+          for (int c = 0; c < NCH; ++c) rd[s][c] = L.raw(Dp, c);
+        }
+        if (care) {
 #pragma unroll
-      for (int c = 0; c < NCH; ++c)
-        rq[s][c] = L.raw((const T*)a.q + i * a.ldq + (int64_t)h * dh, c, ok[s]);
+          for (int s = 0; s < U; ++s)
 #pragma unroll
-      for (int c = 0; c < NCH; ++c)
-        rd[s][c] = L.raw((const T*)a.dout + i * a.lddo + (int64_t)h * dh, c, ok[s]);
-    }
+            for (int c = 0; c < NCH; ++c) {
+              rq[s][c] = L.mask(rq[s][c], c, ok[s] && st[s].x != -INFINITY);
+              rd[s][c] = L.mask(rd[s][c], c, ok[s] && st[s].x != -INFINITY);
+            }
+        }
 #pragma unroll
-    for (int s = 0; s < U; ++s) {
-      float x = 0.f, y = 0.f;
+        for (int s = 0; s < U; ++s) {
+          const float x = head_dot<V, LPH>(kf, rq[s]), y = head_dot<V, LPH>(vf, rd[s]);
+          const float p = ok[s] && st[s].x != -INFINITY
+                              ? __builtin_amdgcn_exp2f(fmaf(x, factor, -st[s].x)) : 0.f;
+          const float ds = p * (y - st[s].y);
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        x = dot<V>(kf[c], rq[s][c], x);
-        y = dot<V>(vf[c], rd[s][c], y);
+          for (int c = 0; c < NCH; ++c) {
+            axpy<V>(ds, rq[s][c], dk[c]);
+            axpy<V>(p, rd[s][c], dv[c]);
+          }
+        }
       }
-      x = group_sum<LPH>(x);
-      y = group_sum<LPH>(y);
-      const float p = ok[s] && st[s].x != -INFINITY ? __builtin_amdgcn_exp2f(x - st[s].x) : 0.f;
-      const float ds = ok[s] ? p * (y - st[s].y) : 0.f;
-#pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        axpy<V>(ds, rq[s][c], dk[c]);
-        axpy<V>(p, rd[s][c], dv[c]);
-      }
     }
+    const float z = on ? zero_of(dk, zero_of(dv, 0.f)) : 0.f;
+    if (care || !__any(z != z)) break;
   }
   for (int w = LPH * hpw; w < 64; w <<= 1) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        dk[c][k] += __shfl_xor(dk[c][k], w, 64);
-        dv[c][k] += __shfl_xor(dv[c][k], w, 64);
+        dk[c][k] += lane_xor(dk[c][k], w);
+        dv[c][k] += lane_xor(dv[c][k], w);
       }
   }
   if (slot != 0 || !on) return;
-  if (pieces) {
+  if (u.slot >= 0) {
     float* part = ws + ((int64_t)u.slot * a.kv_heads + kvh) * (2 * dh);
     L.store(part, dk, 1.f);
     L.store(part + dh, dv, 1.f);
@@ -380,67 +517,75 @@ __global__ __launch_bounds__(256) void k_attn_cols(const gnnea_attn a, int hpw, 
   L.store((T*)a.dv + u.row * a.lddv + (int64_t)kvh * dh, dv, 1.f);
 }
 
-// Joins the pieces of a long row in order: one wave per row and head, a lane per four columns.
+// Joins the pieces of a long row: a workgroup per row and head.  Its waves take the pieces in turn,
+// four columns to a lane; their sums meet in LDS in wave order.
 template <typename T>
-__global__ __launch_bounds__(64) void k_attn_join(const gnnea_attn a, int pass,
-                                                  const float* __restrict__ ws) {
+__global__ __launch_bounds__(512) void k_attn_join(const gnnea_attn a, int pass,
+                                                   const float* __restrict__ ws) {
+  __shared__ float sh[8][2 * 256 + 1];
   const int w = blockIdx.x, h = blockIdx.y, dh = a.d_head, row = a.long_rows[w];
-  const int s0 = a.long_ptr[w], s1 = a.long_ptr[w + 1];
+  const int s0 = a.long_ptr[w], n = a.long_ptr[w + 1] - s0;
+  const bool fwd = pass == GNNEA_ATTN_FWD, rows = pass == GNNEA_ATTN_BWD_ROWS;
   const int heads = pass == GNNEA_ATTN_BWD_COLS ? a.kv_heads : a.heads;
-  const int wide = pass == GNNEA_ATTN_FWD ? dh + 2 : pass == GNNEA_ATTN_BWD_ROWS ? 2 * dh + 1 : 2 * dh;
+  const int wide = fwd ? dh + 2 : rows ? 2 * dh + 1 : 2 * dh;
   const float* part = ws + ((int64_t)s0 * heads + h) * wide;
   const int64_t step = (int64_t)heads * wide;
-  const int n = s1 - s0;
-  if (pass == GNNEA_ATTN_FWD) {
-    float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < n; ++s) {
+  const int lane = lane_id(), wv = wave_id();
+  float m = -INFINITY;
+  if (fwd) {
+    for (int s = lane; s < n; s += 64) {
       const float x = part[s * step];
       m = x > m || x != x ? x : m;
     }
-    const float ref = m == -INFINITY ? 0.f : m;
-    for (int s = 0; s < n; ++s) {
-      const float f = __builtin_amdgcn_exp2f(part[s * step] - ref);
-      sum = fmaf(part[s * step + 1], f, sum);
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (c * 64 + (int)threadIdx.x < dh)
-          o[c] = fmaf(part[s * step + 2 + c * 64 + threadIdx.x], f, o[c]);
+    for (int o = 32; o > 0; o >>= 1) {
+      const float x = __shfl_xor(m, o, 64);
+      m = x > m || x != x ? x : m;
     }
-    const float r = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (c * 64 + (int)threadIdx.x < dh)
-        ((T*)a.o)[row * a.ldo + (int64_t)h * dh + c * 64 + threadIdx.x] = from_f32<T>(o[c] * r);
-    if (a.lse && threadIdx.x == 0)
-      a.lse[(int64_t)row * a.heads + h] = sum == 0.f ? -INFINITY : fmaf(m, kLn2, logf(sum));
-    return;
   }
-  const bool rows = pass == GNNEA_ATTN_BWD_ROWS;
-  float delta = 0.f, A[4] = {0.f, 0.f, 0.f, 0.f}, B[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < n; ++s) {
+  const float ref = m == -INFINITY ? 0.f : m;
+  // what a lane adds up: values lane, lane + 64, ... of a piece after its first words
+  const int skip = fwd ? 2 : rows ? 1 : 0, width = wide - skip;
+  float one = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int s = wv; s < n; s += 8) {
     const float* p = part + s * step;
-    if (rows) delta += *p++;
+    const float f = fwd ? __builtin_amdgcn_exp2f(p[0] - ref) : 1.f;
+    if (skip) one = fmaf(p[skip - 1], f, one);
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (c * 64 + (int)threadIdx.x < dh) {
-        A[c] += p[c * 64 + threadIdx.x];
-        B[c] += p[dh + c * 64 + threadIdx.x];
-      }
+    for (int c = 0; c < 8; ++c)
+      if (c * 64 + lane < width) acc[c] = fmaf(p[skip + c * 64 + lane], f, acc[c]);
   }
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int d = c * 64 + threadIdx.x;
-    if (d >= dh) continue;
-    if (rows) {
-      ((T*)a.dq)[row * a.lddq + (int64_t)h * dh + d] = from_f32<T>(a.scale * fmaf(-delta, B[c], A[c]));
+  for (int c = 0; c < 8; ++c)
+    if (c * 64 + lane < width) sh[wv][1 + c * 64 + lane] = acc[c];
+  if (lane == 0) sh[wv][0] = one;
+  __syncthreads();
+  for (int c = threadIdx.x; c <= width; c += 512) {
+    float s = sh[0][c];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += sh[k][c];
+    sh[0][c] = s;
+  }
+  __syncthreads();
+  one = sh[0][0];
+  const float r = fwd ? (one == 0.f ? 0.f : 1.f / one) : a.scale;
+  for (int d = threadIdx.x; d < dh; d += 512) {
+    const float x = sh[0][1 + d];
+    if (fwd) {
+      ((T*)a.o)[row * a.ldo + (int64_t)h * dh + d] = from_f32<T>(x * r);
+    } else if (rows) {
+      ((T*)a.dq)[row * a.lddq + (int64_t)h * dh + d] = from_f32<T>(r * fmaf(-one, sh[0][1 + dh + d], x));
     } else {
-      ((T*)a.dk)[row * a.lddk + (int64_t)h * dh + d] = from_f32<T>(a.scale * A[c]);
-      ((T*)a.dv)[row * a.lddv + (int64_t)h * dh + d] = from_f32<T>(B[c]);
+      ((T*)a.dk)[row * a.lddk + (int64_t)h * dh + d] = from_f32<T>(r * x);
+      ((T*)a.dv)[row * a.lddv + (int64_t)h * dh + d] = from_f32<T>(sh[0][1 + dh + d]);
     }
   }
-  if (rows && threadIdx.x == 0)
+  if (threadIdx.x != 0) return;
+  if (fwd && a.lse)
+    a.lse[(int64_t)row * a.heads + h] = one == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(one);
+  if (rows)
     *(float2*)(a.stat + 2 * ((int64_t)row * a.heads + h)) =
-        make_float2(a.lse[(int64_t)row * a.heads + h] * kLog2e, delta);
+        make_float2(a.lse[(int64_t)row * a.heads + h], one);
 }
 
 static int attn_check(const gnnea_attn* a, int pass) {
@@ -460,6 +605,7 @@ static int attn_check(const gnnea_attn* a, int pass) {
   if (a->n_cols > 0 && !a->col) return GNNEA_EINVAL;
   if ((!a->q && (!cols || a->n_cols)) || a->ldq < wq) return GNNEA_EINVAL;
   if (((!a->k || !a->v) && (cols || a->n_cols)) || a->ldk < wk || a->ldv < wk) return GNNEA_EINVAL;
+  if (!cols && a->ldk != a->ldv) return GNNEA_EINVAL;  // one offset for both
   if (pass == GNNEA_ATTN_FWD) {
     if (!a->o || a->ldo < wq) return GNNEA_EINVAL;
     return GNNEA_OK;
@@ -477,42 +623,49 @@ static int attn_check(const gnnea_attn* a, int pass) {
 static AttnPlan attn_plan(const gnnea_attn* a, int pass) {
   static const int kShape[7][2] = {{4, 1}, {8, 1}, {8, 2}, {8, 3}, {16, 2}, {16, 3}, {16, 4}};
   const int V = a->dtype == GNNEA_F32 ? 4 : 8;
-  AttnPlan p = {16, 4, 1, 1};
+  AttnPlan p = {16, 4, 1, 1, false};
   for (const auto& s : kShape)
     if (s[0] * s[1] * V >= a->d_head) {
       p.lph = s[0];
       p.nch = s[1];
       break;
     }
+  p.full = p.lph * p.nch * V == a->d_head;
   const int heads = pass == GNNEA_ATTN_BWD_COLS ? a->kv_heads : a->heads;
   while (p.hpw < heads && p.hpw < 64 / p.lph) p.hpw *= 2;
   p.units_y = (heads + p.hpw - 1) / p.hpw;
   return p;
 }
 
-template <typename T, int LPH, int NCH>
-static void attn_launch(const gnnea_attn& a, int pass, const AttnPlan& p, bool pieces, float* ws,
+template <typename T, int LPH, int NCH, bool FULL>
+static void attn_launch(const gnnea_attn& a, int pass, const AttnPlan& p, float* ws,
                         hipStream_t s) {
-  const dim3 grid(div_up(pieces ? a.n_items : a.n_rows, 4), p.units_y);
+  const dim3 grid(div_up((int64_t)a.n_items + a.n_rows, 4), p.units_y);
   if (pass == GNNEA_ATTN_FWD)
-    hipLaunchKernelGGL((k_attn_fwd<T, LPH, NCH>), grid, dim3(256), 0, s, a, p.hpw, pieces, ws);
+    hipLaunchKernelGGL((k_attn_fwd<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, p.hpw, ws);
   else if (pass == GNNEA_ATTN_BWD_ROWS)
-    hipLaunchKernelGGL((k_attn_rows<T, LPH, NCH>), grid, dim3(256), 0, s, a, p.hpw, pieces, ws);
+    hipLaunchKernelGGL((k_attn_rows<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, p.hpw, ws);
   else
-    hipLaunchKernelGGL((k_attn_cols<T, LPH, NCH>), grid, dim3(256), 0, s, a, p.hpw, pieces, ws);
+    hipLaunchKernelGGL((k_attn_cols<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, p.hpw, ws);
+}
+template <typename T, int LPH, int NCH>
+static void attn_launch(const gnnea_attn& a, int pass, const AttnPlan& p, float* ws,
+                        hipStream_t s) {
+  if (p.full) attn_launch<T, LPH, NCH, true>(a, pass, p, ws, s);
+  else attn_launch<T, LPH, NCH, false>(a, pass, p, ws, s);
 }
 
 template <typename T>
-static void attn_dispatch(const gnnea_attn& a, int pass, bool pieces, float* ws, hipStream_t s) {
+static void attn_dispatch(const gnnea_attn& a, int pass, float* ws, hipStream_t s) {
   const AttnPlan p = attn_plan(&a, pass);
-  if (p.lph == 4) attn_launch<T, 4, 1>(a, pass, p, pieces, ws, s);
-  else if (p.lph == 8 && p.nch == 1) attn_launch<T, 8, 1>(a, pass, p, pieces, ws, s);
-  else if (p.lph == 8 && p.nch == 2) attn_launch<T, 8, 2>(a, pass, p, pieces, ws, s);
-  else if (p.lph == 8) attn_launch<T, 8, 3>(a, pass, p, pieces, ws, s);
-  else if (p.nch == 2) attn_launch<T, 16, 2>(a, pass, p, pieces, ws, s);
+  if (p.lph == 4) attn_launch<T, 4, 1>(a, pass, p, ws, s);
+  else if (p.lph == 8 && p.nch == 1) attn_launch<T, 8, 1>(a, pass, p, ws, s);
+  else if (p.lph == 8 && p.nch == 2) attn_launch<T, 8, 2>(a, pass, p, ws, s);
+  else if (p.lph == 8) attn_launch<T, 8, 3>(a, pass, p, ws, s);
+  else if (p.nch == 2) attn_launch<T, 16, 2>(a, pass, p, ws, s);
   else if constexpr (sizeof(T) == 4) {  // bf16 heads of 256 fit two chunks
-    if (p.nch == 3) attn_launch<T, 16, 3>(a, pass, p, pieces, ws, s);
-    else attn_launch<T, 16, 4>(a, pass, p, pieces, ws, s);
+    if (p.nch == 3) attn_launch<T, 16, 3>(a, pass, p, ws, s);
+    else attn_launch<T, 16, 4>(a, pass, p, ws, s);
   }
 }
 
@@ -529,17 +682,15 @@ static int attn_run(const gnnea_attn* a, int pass, void* ws, int64_t ws_bytes, v
   if (ws_bytes < attn_ws(a, pass)) return GNNEA_EWORKSPACE;
   if (a->n_items && (!ws || ((uintptr_t)ws & 15))) return ws ? GNNEA_EALIGN : GNNEA_EINVAL;
   const hipStream_t s = (hipStream_t)stream;
-  for (int pieces = 0; pieces < (a->n_items ? 2 : 1); ++pieces) {
-    if (a->dtype == GNNEA_F32) attn_dispatch<float>(*a, pass, pieces, (float*)ws, s);
-    else attn_dispatch<bf16_t>(*a, pass, pieces, (float*)ws, s);
-    GNNEA_LAUNCH_CHECK();
-  }
+  if (a->dtype == GNNEA_F32) attn_dispatch<float>(*a, pass, (float*)ws, s);
+  else attn_dispatch<bf16_t>(*a, pass, (float*)ws, s);
+  GNNEA_LAUNCH_CHECK();
   if (a->n_items) {
     const dim3 grid(a->n_long, pass == GNNEA_ATTN_BWD_COLS ? a->kv_heads : a->heads);
     if (a->dtype == GNNEA_F32)
-      hipLaunchKernelGGL(k_attn_join<float>, grid, dim3(64), 0, s, *a, pass, (const float*)ws);
+      hipLaunchKernelGGL(k_attn_join<float>, grid, dim3(512), 0, s, *a, pass, (const float*)ws);
     else
-      hipLaunchKernelGGL(k_attn_join<bf16_t>, grid, dim3(64), 0, s, *a, pass, (const float*)ws);
+      hipLaunchKernelGGL(k_attn_join<bf16_t>, grid, dim3(512), 0, s, *a, pass, (const float*)ws);
     GNNEA_LAUNCH_CHECK();
   }
   return 0;

@@ -39,32 +39,66 @@ __device__ __forceinline__ Gate gate_of(float z) {
   return z >= 0.f ? Gate{r, e * r} : Gate{e * r, r};
 }
 
-// V weights of either type from column c on (fp32 weights beside bf16 features: two 16-B loads)
-template <typename TW, int V>
-__device__ __forceinline__ void load_vec(const TW* p, int left, float (&f)[V], float none) {
-  if (!p) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) f[k] = none;
-    return;
+// value c of a vector of either type, `none` where there is none
+__device__ __forceinline__ float vec_at(const void* p, bool bf16, int c, float none) {
+  if (!p) return none;
+  return bf16 ? bf16_to_f32(((const bf16_t*)p)[c]) : ((const float*)p)[c];
+}
+
+// The columns of a thread: chunk i of NIT begins at column (i TPR + t) V; the last chunk of a row
+// is moved back so that it ends with the row (its first values are then the neighbour's too, who
+// computes and stores the same; the sums take each once).
+template <int TPR, int NIT, int V> struct Cols {
+  int D, t;
+  __device__ __forceinline__ int want(int i) const {
+    return (i * (TPR < 256 ? TPR : (int)blockDim.x) + t) * V;
   }
-  if constexpr (RowChunk<TW>::V == V) {
-    load_chunk<TW, V>(p, left, f);
-  } else if (left >= V) {
-    const uint4 a = load16<TW>(p), b = load16<TW>(p + 4);
-    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = __builtin_bit_cast(float, w[k]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k) f[k] = k < left ? to_f32<TW>(p[k]) : 0.f;
+  __device__ __forceinline__ bool has(int i) const { return want(i) < D; }
+  __device__ __forceinline__ int at(int i) const {
+    const int c = want(i);
+    return D >= V && c > D - V ? D - V : c;
   }
+  // whether value k of chunk i is the thread's own: all are, but in a row's last chunk
+  __device__ __forceinline__ bool own(int i, int k) const {
+    if (i < NIT - 1) return true;
+    if (TPR == 16 && k >= D) return false;
+    return k >= (has(i) ? want(i) - at(i) : V);
+  }
+};
+
+template <typename T, int TPR, int NIT, int V>
+__device__ __forceinline__ void load_row(const Cols<TPR, NIT, V>& C, const T* p, uint4 (&r)[NIT]) {
+#pragma unroll
+  for (int i = 0; i < NIT; ++i) {
+    r[i] = make_uint4(0, 0, 0, 0);
+    if (!C.has(i)) continue;
+    if (TPR > 16 || C.D >= V) {
+      r[i] = load16<T>(p + C.at(i));
+    } else {  // rows narrower than 16 B (one thread per row)
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        if (k < C.D) {
+          if constexpr (V == 4) w[k] = __builtin_bit_cast(uint32_t, (float)to_f32<T>(p[k]));
+          else w[k / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[k]) << (16 * (k & 1));
+        }
+      r[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+template <typename T, int TPR, int NIT, int V>
+__device__ __forceinline__ void store_row(const Cols<TPR, NIT, V>& C, T* p, int i,
+                                          const float (&f)[V]) {
+  if (!C.has(i)) return;
+  if (TPR > 16 || C.D >= V) store_chunk<T, V>(p + C.at(i), V, f);
+  else store_chunk<T, V>(p, C.D, f);
 }
 
 // Sums of NS values over the TPR threads of a row; every thread gets them, from the same order of
 // additions.  16 lanes and a wave stay in registers; a workgroup goes once through LDS (two
 // buffers in turn, so one barrier per sum is enough).
 template <int TPR, int NS>
-__device__ __forceinline__ void row_sum(float (&v)[NS], float (*sh)[8][NS], int& turn) {
+__device__ __forceinline__ void row_sum(float (&v)[NS], float (*sh)[16][2], int& turn) {
 #pragma unroll
   for (int k = 0; k < NS; ++k) {
     v[k] += mov_dpp_f32<0xB1>(v[k]);
@@ -76,7 +110,7 @@ __device__ __forceinline__ void row_sum(float (&v)[NS], float (*sh)[8][NS], int&
              readlane_f(v[k], 48);
   }
   if constexpr (TPR > 64) {
-    float(*b)[NS] = sh[turn];
+    float(*b)[2] = sh[turn];
     turn ^= 1;
     if (lane_id() == 0) {
 #pragma unroll
@@ -86,183 +120,267 @@ __device__ __forceinline__ void row_sum(float (&v)[NS], float (*sh)[8][NS], int&
 #pragma unroll
     for (int k = 0; k < NS; ++k) {
       float s = b[0][k];
-#pragma unroll
-      for (int w = 1; w < TPR / 64; ++w) s += b[w][k];
+      for (int w = 1; w < (int)blockDim.x / 64; ++w) s += b[w][k];
       v[k] = s;
     }
   }
 }
 
-// mean and 1 / sqrt(var + eps) (0 and 1 / rms) of the row's values f
+// mean and 1 / sqrt(var + eps) (0 and 1 / rms) of the row's values f.  LayerNorm in a workgroup:
+// each wave sums its values, then their squares about its own mean, and the waves' pairs are put
+// together about the row's mean (one barrier instead of two, and no difference of large sums).
 template <int TPR, int NIT, int V>
-__device__ __forceinline__ void row_stats(const float (&f)[NIT][V], int D, int c0, bool layer,
-                                          float eps, float (*sh)[8][1], int& turn, float& mean,
-                                          float& rho) {
+__device__ __forceinline__ void row_stats(const Cols<TPR, NIT, V>& C, const float (&f)[NIT][V],
+                                          float inv, bool layer, float eps, float (*sh)[16][2],
+                                          const float* share, int& turn, float& mean, float& rho) {
   mean = 0.f;
-  float s[1];
+  float s[1] = {0.f}, count = 0.f;
+  int none = 0;
   if (layer) {
-    s[0] = 0.f;
 #pragma unroll
     for (int i = 0; i < NIT; ++i)
 #pragma unroll
-      for (int k = 0; k < V; ++k) s[0] += f[i][k];  // places past the row hold 0
-    row_sum<TPR, 1>(s, sh, turn);
-    mean = s[0] / (float)D;
+      for (int k = 0; k < V; ++k) s[0] += C.own(i, k) ? f[i][k] : 0.f;
+    row_sum<(TPR < 64 ? TPR : 64), 1>(s, sh, none);
+    if constexpr (TPR > 64) count = share[wave_id()];
+    mean = s[0] * (TPR > 64 ? (count > 0.f ? 1.f / count : 0.f) : inv);
   }
   s[0] = 0.f;
 #pragma unroll
   for (int i = 0; i < NIT; ++i)
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const float d = c0 + i * TPR * V + k < D ? f[i][k] - mean : 0.f;
+      const float d = C.own(i, k) ? f[i][k] - mean : 0.f;
       s[0] = fmaf(d, d, s[0]);
     }
-  row_sum<TPR, 1>(s, sh, turn);
-  rho = 1.f / sqrtf(s[0] / (float)D + eps);
+  if constexpr (TPR <= 64) {
+    row_sum<TPR, 1>(s, sh, none);
+  } else if (!layer) {
+    row_sum<TPR, 1>(s, sh, turn);
+  } else {
+    float w[1] = {s[0]};
+    row_sum<64, 1>(w, sh, none);
+    float(*b)[2] = sh[turn];
+    turn ^= 1;
+    if (lane_id() == 0) b[wave_id()][0] = mean, b[wave_id()][1] = w[0];
+    __syncthreads();
+    const int waves = blockDim.x / 64;
+    mean = 0.f;
+    for (int q = 0; q < waves; ++q) mean = fmaf(b[q][0], share[q], mean);
+    mean *= inv;
+    s[0] = 0.f;
+    for (int q = 0; q < waves; ++q) {
+      const float d = b[q][0] - mean;
+      s[0] += fmaf(d * d, share[q], b[q][1]);
+    }
+  }
+  rho = __builtin_amdgcn_rsqf(fmaf(s[0], inv, eps));
 }
 
-template <typename T, typename TW, int TPR, int NIT>
+// the number of a row's values that each wave of the workgroup holds
+template <int TPR, int NIT, int V>
+__device__ __forceinline__ void wave_shares(const Cols<TPR, NIT, V>& C, float* share) {
+  if constexpr (TPR > 64) {
+    if (threadIdx.x < 16) {
+      int n = 0;
+      for (int i = 0; i < NIT; ++i)
+        n += max(0, min(64 * V, C.D - (i * (int)blockDim.x + (int)threadIdx.x * 64) * V));
+      share[threadIdx.x] = (float)n;
+    }
+    __syncthreads();
+  }
+}
+
+// IN: 0: no y; 1: y; 2: y and a gate of its own for every element (a gate shared by all rows is
+// part of the thread's constants: P = alpha scale g post_w, Q = alpha scale g post_b)
+template <typename T, int TPR, int NIT, int IN>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const gnnea_norm a) {
-  constexpr int V = RowChunk<T>::V;
-  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
-  __shared__ float sh[2][8][1];
+  constexpr int V = RowChunk<T>::V, RPB = TPR < 256 ? 256 / TPR : 1;
+  __shared__ float sh[2][16][2];
   int turn = 0;
-  const int D = a.D, t = threadIdx.x % TPR, c0 = t * V;
-  const bool layer = a.kind == GNNEA_NORM_LAYER;
-  const T* __restrict__ X = (const T*)a.x;
-  const T* __restrict__ Y = (const T*)a.y;
-  const T* __restrict__ Z = (const T*)a.gate;
-  const TW* __restrict__ W = (const TW*)a.post_w;
-  const TW* __restrict__ Bv = (const TW*)a.post_b;
-  const TW* __restrict__ S = (const TW*)a.scale;
-  const TW* __restrict__ W2 = (const TW*)a.pre_w;
-  const TW* __restrict__ B2 = (const TW*)a.pre_b;
-  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < a.n;
-       row += (int64_t)gridDim.x * RPB) {
+  const Cols<TPR, NIT, V> C{a.D, (int)(threadIdx.x % (TPR < 256 ? TPR : 1024))};
+  const bool layer = a.kind == GNNEA_NORM_LAYER, wb = a.w_dtype == GNNEA_BF16;
+  const float inv = 1.f / (float)a.D;
+  __shared__ float share[16];
+  wave_shares(C, share);
+  float P[NIT][V], Q[NIT][V], W[NIT][V], B[NIT][V];
+#pragma unroll
+  for (int i = 0; i < NIT; ++i)
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int c = min(C.at(i) + k, a.D - 1);
+      if constexpr (IN) {
+        float s = a.alpha * vec_at(a.scale, wb, c, 1.f);
+        if (a.gate_mode == GNNEA_GATE_ROW) s *= gate_of(vec_at(a.gate, wb, c, 0.f)).g;
+        P[i][k] = s * vec_at(a.post_w, wb, c, 1.f);
+        Q[i][k] = s * vec_at(a.post_b, wb, c, 0.f);
+      }
+      W[i][k] = vec_at(a.pre_w, wb, c, 1.f);
+      B[i][k] = vec_at(a.pre_b, wb, c, 0.f);
+    }
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  uint4 rx[NIT], ry[NIT], rz[NIT];
+  auto load = [&](int64_t at) {
+    load_row<T>(C, (const T*)a.x + at * a.ldx, rx);
+    if constexpr (IN) load_row<T>(C, (const T*)a.y + at * a.ldy, ry);
+    if constexpr (IN == 2) load_row<T>(C, (const T*)a.gate + at * a.ldg, rz);
+  };
+  if (row < a.n) load(row);
+  for (; row < a.n; row += step) {
     float r[NIT][V], y[NIT][V], z[NIT][V];
 #pragma unroll
     for (int i = 0; i < NIT; ++i) {
-      const int c = c0 + i * TPR * V;
-      load_chunk<T, V>(X + row * a.ldx + c, D - c, r[i]);
-      if (Y) load_chunk<T, V>(Y + row * a.ldy + c, D - c, y[i]);
-      if (a.gate_mode == GNNEA_GATE_FULL)
-        load_chunk<T, V>(Z + row * a.ldg + c, D - c, z[i]);
-      else if (a.gate_mode == GNNEA_GATE_ROW)
-        load_vec<TW, V>((const TW*)a.gate + c, D - c, z[i], 0.f);
+      unpack16(rx[i], r[i]);
+      if constexpr (IN) unpack16(ry[i], y[i]);
+      if constexpr (IN == 2) unpack16(rz[i], z[i]);
     }
+    if (row + step < a.n) load(row + step);  // on its way while this row is computed
     float mean = 0.f, rho = 1.f, mean2 = 0.f, rho2 = 1.f;
-    if (Y) {
-      if (a.post) row_stats<TPR, NIT, V>(y, D, c0, layer, a.eps, sh, turn, mean, rho);
+    if constexpr (IN) {
+      if (a.post) row_stats(C, y, inv, layer, a.eps, sh, share, turn, mean, rho);
 #pragma unroll
       for (int i = 0; i < NIT; ++i) {
-        const int c = c0 + i * TPR * V;
-        float w[V], b[V], s[V];
-        load_vec<TW, V>(W ? W + c : W, D - c, w, 1.f);
-        load_vec<TW, V>(Bv ? Bv + c : Bv, D - c, b, 0.f);
-        load_vec<TW, V>(S ? S + c : S, D - c, s, 1.f);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float u = fmaf((y[i][k] - mean) * rho, w[k], b[k]);
-          const float g = a.gate_mode ? gate_of(z[i][k]).g : 1.f;
-          r[i][k] = c + k < D ? fmaf(a.alpha * s[k] * g, u, r[i][k]) : 0.f;
+          const float u = fmaf((y[i][k] - mean) * rho, P[i][k], Q[i][k]);
+          if constexpr (IN == 2) r[i][k] = fmaf(gate_of(z[i][k]).g, u, r[i][k]);
+          else r[i][k] += u;
         }
-        if (a.r) store_chunk<T, V>((T*)a.r + row * a.ldr + c, D - c, r[i]);
+        store_row<T>(C, (T*)a.r + row * a.ldr, i, r[i]);
       }
     }
     if (a.pre) {
-      row_stats<TPR, NIT, V>(r, D, c0, layer, a.eps, sh, turn, mean2, rho2);
+      row_stats(C, r, inv, layer, a.eps, sh, share, turn, mean2, rho2);
 #pragma unroll
       for (int i = 0; i < NIT; ++i) {
-        const int c = c0 + i * TPR * V;
-        float w[V], b[V];
-        load_vec<TW, V>(W2 ? W2 + c : W2, D - c, w, 1.f);
-        load_vec<TW, V>(B2 ? B2 + c : B2, D - c, b, 0.f);
+        float h[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) r[i][k] = fmaf((r[i][k] - mean2) * rho2, w[k], b[k]);
-        store_chunk<T, V>((T*)a.h + row * a.ldh + c, D - c, r[i]);
+        for (int k = 0; k < V; ++k) h[k] = fmaf((r[i][k] - mean2) * rho2, W[i][k], B[i][k]);
+        store_row<T>(C, (T*)a.h + row * a.ldh, i, h);
       }
     }
-    if (a.stats && t == 0)
+    if (a.stats && C.t == 0)
       *(float4*)(a.stats + 4 * row) = make_float4(mean, rho, mean2, rho2);
   }
 }
 
-template <typename T, typename TW, int TPR, int NIT>
+// BIAS: post_b or pre_b takes part (without them the sums B and E are not formed)
+template <typename T, int TPR, int NIT, int IN, bool BIAS>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_norm a) {
-  constexpr int V = RowChunk<T>::V;
-  constexpr int NT = TPR < 256 ? 256 : TPR;
-  constexpr int RPB = NT / TPR;
-  __shared__ float sh[2][8][2];
-  __shared__ float fold[RPB > 1 ? NT * NIT * V : 1];
+  // the next row is read while this one is computed, where registers allow it (1024 threads with a
+  // full gate have none left)
+  constexpr bool kAhead = TPR <= 512 || IN < 2;
+  constexpr int V = RowChunk<T>::V, RPB = TPR < 256 ? 256 / TPR : 1;
+  __shared__ float sh[2][16][2];
+  // the column sums: in registers, or (rows of a workgroup, whose registers are short) in LDS,
+  // every thread its own places
+  constexpr bool kLds = TPR > 64;
+  constexpr int kHeld = kLds ? 1 : kNormSums;
+  extern __shared__ float fold[];
   int turn = 0;
-  const int D = a.D, t = threadIdx.x % TPR, c0 = t * V;
-  const bool layer = a.kind == GNNEA_NORM_LAYER;
-  const float inv = 1.f / (float)D;
-  const T* __restrict__ X = (const T*)a.x;
-  const T* __restrict__ Y = (const T*)a.y;
-  const T* __restrict__ Z = (const T*)a.gate;
-  const T* __restrict__ DR = (const T*)a.dr;
-  const T* __restrict__ DH = (const T*)a.dh;
-  const TW* __restrict__ W = (const TW*)a.post_w;
-  const TW* __restrict__ Bv = (const TW*)a.post_b;
-  const TW* __restrict__ S = (const TW*)a.scale;
-  const TW* __restrict__ W2 = (const TW*)a.pre_w;
-  float acc[kNormSums][NIT][V];
+  const Cols<TPR, NIT, V> C{a.D, (int)(threadIdx.x % (TPR < 256 ? TPR : 1024))};
+  const bool layer = a.kind == GNNEA_NORM_LAYER, wb = a.w_dtype == GNNEA_BF16;
+  const float inv = 1.f / (float)a.D;
+  float P[NIT][V], Q[NIT][V], W[NIT][V], acc[kHeld][NIT][V];
 #pragma unroll
-  for (int q = 0; q < kNormSums; ++q)
+  for (int i = 0; i < NIT; ++i)
 #pragma unroll
-    for (int i = 0; i < NIT; ++i)
+    for (int k = 0; k < V; ++k) {
+      const int c = min(C.at(i) + k, a.D - 1);
+      if constexpr (IN) {
+        float s = a.alpha * vec_at(a.scale, wb, c, 1.f);
+        if (a.gate_mode == GNNEA_GATE_ROW) s *= gate_of(vec_at(a.gate, wb, c, 0.f)).g;
+        P[i][k] = s * vec_at(a.post_w, wb, c, 1.f);
+        Q[i][k] = BIAS ? s * vec_at(a.post_b, wb, c, 0.f) : 0.f;
+      }
+      W[i][k] = vec_at(a.pre_w, wb, c, 1.f);
 #pragma unroll
-      for (int k = 0; k < V; ++k) acc[q][i][k] = 0.f;
-  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < a.n;
-       row += (int64_t)gridDim.x * RPB) {
-    const float4 st = *(const float4*)(a.stats + 4 * row);
+      for (int q = 0; q < kHeld; ++q) acc[q][i][k] = 0.f;
+    }
+  // four values of a sum at a time, the threads' next to each other
+  const int nt = blockDim.x;
+  float4* held = (float4*)fold + threadIdx.x;
+  if constexpr (kLds) {
+#pragma unroll
+    for (int j = 0; j < kNormSums * NIT * V / 4; ++j) held[j * nt] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  // sum q of the columns of chunk i: + x y
+  auto add = [&](int q, int i, const float (&x)[V], const float (&y)[V]) {
+    if constexpr (kLds) {
+#pragma unroll
+      for (int j = 0; j < V / 4; ++j) {
+        float4* p = held + ((q * NIT + i) * (V / 4) + j) * nt;
+        float4 f = *p;
+        f.x = fmaf(x[4 * j], y[4 * j], f.x);
+        f.y = fmaf(x[4 * j + 1], y[4 * j + 1], f.y);
+        f.z = fmaf(x[4 * j + 2], y[4 * j + 2], f.z);
+        f.w = fmaf(x[4 * j + 3], y[4 * j + 3], f.w);
+        *p = f;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[q][i][k] = fmaf(x[k], y[k], acc[q][i][k]);
+    }
+  };
+  float ones[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) ones[k] = 1.f;
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  uint4 rx[NIT], ry[NIT], rz[NIT], rd[NIT], rm[NIT];
+  float4 rs;
+#pragma unroll
+  for (int i = 0; i < NIT; ++i) rd[i] = rm[i] = make_uint4(0, 0, 0, 0);
+  auto load = [&](int64_t at) {
+    rs = *(const float4*)(a.stats + 4 * at);
+    load_row<T>(C, (const T*)a.x + at * a.ldx, rx);
+    if constexpr (IN) load_row<T>(C, (const T*)a.y + at * a.ldy, ry);
+    if constexpr (IN == 2) load_row<T>(C, (const T*)a.gate + at * a.ldg, rz);
+    if (a.dr) load_row<T>(C, (const T*)a.dr + at * a.lddr, rd);
+    if (a.dh) load_row<T>(C, (const T*)a.dh + at * a.lddh, rm);
+  };
+  if (kAhead && row < a.n) load(row);
+  for (; row < a.n; row += step) {
+    if (!kAhead) load(row);
     // n: the normalised y;  r: the normalised residual row, later q;  z: the gate's argument, later
     // its gradient;  d: dr, later dx;  m: dh, later dh w'
     float n[NIT][V], r[NIT][V], z[NIT][V], d[NIT][V], m[NIT][V];
+    const float4 st = rs;
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+      unpack16(rx[i], r[i]);
+      if constexpr (IN) unpack16(ry[i], n[i]);
+      if constexpr (IN == 2) unpack16(rz[i], z[i]);
+      unpack16(rd[i], d[i]);
+      unpack16(rm[i], m[i]);
+    }
+    if (kAhead && row + step < a.n) load(row + step);
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NIT; ++i) {
-      const int c = c0 + i * TPR * V;
-      load_chunk<T, V>(X + row * a.ldx + c, D - c, r[i]);
-      if (Y) load_chunk<T, V>(Y + row * a.ldy + c, D - c, n[i]);
-      if (a.gate_mode == GNNEA_GATE_FULL)
-        load_chunk<T, V>(Z + row * a.ldg + c, D - c, z[i]);
-      else if (a.gate_mode == GNNEA_GATE_ROW)
-        load_vec<TW, V>((const TW*)a.gate + c, D - c, z[i], 0.f);
-      if (DR) load_chunk<T, V>(DR + row * a.lddr + c, D - c, d[i]);
-      if (DH) load_chunk<T, V>(DH + row * a.lddh + c, D - c, m[i]);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        if (!DR) d[i][k] = 0.f;
-        if (!DH) m[i][k] = 0.f;
-        if (!Y) n[i][k] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NIT; ++i) {
-      const int c = c0 + i * TPR * V;
-      float w[V], b[V], s[V], w2[V];
-      load_vec<TW, V>(W ? W + c : W, D - c, w, 1.f);
-      load_vec<TW, V>(Bv ? Bv + c : Bv, D - c, b, 0.f);
-      load_vec<TW, V>(S ? S + c : S, D - c, s, 1.f);
-      load_vec<TW, V>(W2 ? W2 + c : W2, D - c, w2, 1.f);
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        if (Y) {
-          const float g = a.gate_mode ? gate_of(z[i][k]).g : 1.f;
+        if constexpr (IN) {
           n[i][k] = (n[i][k] - st.x) * st.y;
-          r[i][k] = fmaf(a.alpha * s[k] * g, fmaf(n[i][k], w[k], b[k]), r[i][k]);
+          const float u = fmaf(n[i][k], P[i][k], Q[i][k]);
+          if constexpr (IN == 2) r[i][k] = fmaf(gate_of(z[i][k]).g, u, r[i][k]);
+          else r[i][k] += u;
         }
-        r[i][k] = (r[i][k] - st.z) * st.w;  // the normalised residual row
-        acc[2][i][k] = fmaf(m[i][k], r[i][k], acc[2][i][k]);
-        acc[3][i][k] += m[i][k];
-        m[i][k] *= w2[k];
-        sum[0] += m[i][k];  // m is 0 past the row
-        sum[1] = fmaf(m[i][k], r[i][k], sum[1]);
+        r[i][k] = (r[i][k] - st.z) * st.w;
+        // (values of the neighbour's columns go into sums that are not written)
+      }
+      add(2, i, m[i], r[i]);
+      if constexpr (BIAS) add(3, i, m[i], ones);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        m[i][k] *= W[i][k];
+        const float q = C.own(i, k) ? m[i][k] : 0.f;
+        sum[0] += q;
+        sum[1] = fmaf(q, r[i][k], sum[1]);
       }
     }
-    if (DH) {
+    if (a.dh) {
       row_sum<TPR, 2>(sum, sh, turn);
       const float m0 = layer ? sum[0] * inv : 0.f, m1 = sum[1] * inv;
 #pragma unroll
@@ -274,29 +392,28 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
     sum[0] = sum[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < NIT; ++i) {
-      const int c = c0 + i * TPR * V;
-      if (a.dx) store_chunk<T, V>((T*)a.dx + row * a.lddx + c, D - c, d[i]);
-      if (!Y) continue;
-      float w[V], b[V], s[V];
-      load_vec<TW, V>(W ? W + c : W, D - c, w, 1.f);
-      load_vec<TW, V>(Bv ? Bv + c : Bv, D - c, b, 0.f);
-      load_vec<TW, V>(S ? S + c : S, D - c, s, 1.f);
+      if (a.dx) store_row<T>(C, (T*)a.dx + row * a.lddx, i, d[i]);
+      if constexpr (IN) {
+        float dg[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float u = fmaf(n[i][k], w[k], b[k]);
-        const Gate g = a.gate_mode ? gate_of(z[i][k]) : Gate{1.f, 0.f};
-        const float dg = c + k < D ? d[i][k] * g.g : 0.f, sd = a.alpha * s[k] * dg;
-        acc[0][i][k] = fmaf(dg, n[i][k], acc[0][i][k]);
-        acc[1][i][k] += dg;
-        z[i][k] = sd * u * g.rest;
-        r[i][k] = sd * w[k];
-        sum[0] += r[i][k];
-        sum[1] = fmaf(r[i][k], n[i][k], sum[1]);
+        for (int k = 0; k < V; ++k) {
+          dg[k] = d[i][k];
+          if constexpr (IN == 2) {
+            const Gate g = gate_of(z[i][k]);
+            dg[k] *= g.g;
+            z[i][k] = dg[k] * g.rest * fmaf(n[i][k], P[i][k], Q[i][k]);
+          }
+          r[i][k] = dg[k] * P[i][k];
+          const float q = C.own(i, k) ? r[i][k] : 0.f;
+          sum[0] += q;
+          sum[1] = fmaf(q, n[i][k], sum[1]);
+        }
+        add(0, i, dg, n[i]);
+        if constexpr (BIAS) add(1, i, dg, ones);
+        if (IN == 2 && a.dgate) store_row<T>(C, (T*)a.dgate + row * a.lddg, i, z[i]);
       }
-      if (a.gate_mode == GNNEA_GATE_FULL && a.dgate)
-        store_chunk<T, V>((T*)a.dgate + row * a.lddg + c, D - c, z[i]);
     }
-    if (Y && a.dy) {
+    if (IN && a.dy) {
       float q0 = 0.f, q1 = 0.f;
       if (a.post) {
         row_sum<TPR, 2>(sum, sh, turn);
@@ -305,10 +422,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
       }
 #pragma unroll
       for (int i = 0; i < NIT; ++i) {
-        const int c = c0 + i * TPR * V;
 #pragma unroll
         for (int k = 0; k < V; ++k) r[i][k] = st.y * (r[i][k] - q0 - n[i][k] * q1);
-        store_chunk<T, V>((T*)a.dy + row * a.lddy + c, D - c, r[i]);
+        store_row<T>(C, (T*)a.dy + row * a.lddy, i, r[i]);
       }
     }
   }
@@ -317,97 +433,115 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
 #pragma unroll
   for (int q = 0; q < kNormSums; ++q) {
     if (!(a.sums & (1 << q))) continue;
-    float* out = a.part + ((int64_t)blockIdx.x * kNormSums + q) * D;
+    float* out = a.part + ((int64_t)blockIdx.x * kNormSums + q) * C.D;
     if constexpr (RPB == 1) {
-#pragma unroll
-      for (int i = 0; i < NIT; ++i) {
-        const int c = c0 + i * TPR * V;
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (c + k < D) out[c + k] = acc[q][i][k];
-      }
-    } else {
-      __syncthreads();
-      const int rid = threadIdx.x / TPR;
 #pragma unroll
       for (int i = 0; i < NIT; ++i)
 #pragma unroll
-        for (int k = 0; k < V; ++k) fold[rid * (TPR * NIT * V) + c0 + i * TPR * V + k] = acc[q][i][k];
+        for (int k = 0; k < V; ++k)
+          if (C.has(i) && C.own(i, k))
+            out[C.at(i) + k] =
+                fold[(((q * NIT + i) * (V / 4) + k / 4) * nt + threadIdx.x) * 4 + k % 4];
+    } else {
+      constexpr int kRow = TPR * NIT * V;  // (of LDS, for each of the workgroup's rows)
       __syncthreads();
-      for (int c = threadIdx.x; c < D; c += NT) {
+#pragma unroll
+      for (int i = 0; i < NIT; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (C.has(i) && C.own(i, k))
+            fold[(threadIdx.x / TPR) * kRow + C.at(i) + k] = acc[q][i][k];
+      __syncthreads();
+      for (int c = threadIdx.x; c < C.D; c += 256) {
         float s = fold[c];
-        for (int w = 1; w < RPB; ++w) s += fold[w * (TPR * NIT * V) + c];
+        for (int w = 1; w < RPB; ++w) s += fold[w * kRow + c];
         out[c] = s;
       }
     }
   }
 }
 
-// The workgroups' column sums in workgroup order (fp64), and the six vector gradients from them.
-// 64 columns per workgroup, 16 waves take every 16th partial row.
-template <typename TW>
+// The workgroups' column sums in a fixed order (fp64), and the six vector gradients from them.  16
+// columns per workgroup; 64 groups of 16 lanes take every 64th partial row.
 __global__ __launch_bounds__(1024) void k_norm_fold(const gnnea_norm a, int blocks) {
-  __shared__ double sh[16][64];
-  const int c = blockIdx.x * 64 + lane_id(), w = wave_id();
-  const bool in = c < a.D;
+  __shared__ double sh[kNormSums][64][17];
+  const int lc = threadIdx.x & 15, w = threadIdx.x >> 4, c = blockIdx.x * 16 + lc;
+  const bool in = c < a.D, wb = a.w_dtype == GNNEA_BF16;
+  double s[kNormSums] = {0.0, 0.0, 0.0, 0.0};
+  float scale = 0.f, gate = 0.f, pw = 0.f, pb = 0.f;
+  if (in) {
+    scale = a.alpha * vec_at(a.scale, wb, c, 1.f);
+    gate = a.gate_mode == GNNEA_GATE_ROW ? vec_at(a.gate, wb, c, 0.f) : 0.f;
+    pw = vec_at(a.post_w, wb, c, 1.f);
+    pb = vec_at(a.post_b, wb, c, 0.f);
+    for (int b = w; b < blocks; b += 64 * 4) {
+      float v[4][kNormSums];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int q = 0; q < kNormSums; ++q)
+          v[u][q] = (a.sums & (1 << q)) && b + 64 * u < blocks
+                        ? a.part[((int64_t)(b + 64 * u) * kNormSums + q) * a.D + c] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int q = 0; q < kNormSums; ++q) s[q] += (double)v[u][q];
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < kNormSums; ++q) sh[q][w][lc] = s[q];
+  __syncthreads();
+  if (threadIdx.x < 64) {  // 16 columns x the four sums
+    const int q = threadIdx.x >> 4;
+    double t = sh[q][0][lc];
+    for (int k = 1; k < 64; ++k) t += sh[q][k][lc];
+    sh[q][0][lc] = t;
+  }
+  __syncthreads();
+  if (threadIdx.x >= 16 || !in) return;
   float got[kNormSums];
 #pragma unroll
-  for (int q = 0; q < kNormSums; ++q) {
-    got[q] = 0.f;
-    if (!(a.sums & (1 << q))) continue;
-    double s = 0.0;
-    if (in) {
-      const float* p = a.part + (int64_t)q * a.D + c;
-      const int64_t step = (int64_t)kNormSums * a.D;
-      int b = w;
-      for (; b + 112 < blocks; b += 128) {
-        float v[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = p[(b + 16 * u) * step];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) s += (double)v[u];
-      }
-      for (; b < blocks; b += 16) s += (double)p[b * step];
-    }
-    __syncthreads();
-    sh[w][lane_id()] = s;
-    __syncthreads();
-    if (w == 0) {
-      for (int k = 1; k < 16; ++k) s += sh[k][lane_id()];
-      got[q] = (float)s;
-    }
-  }
-  if (w != 0 || !in) return;
-  const float pw = a.post_w ? to_f32<TW>(((const TW*)a.post_w)[c]) : 1.f;
-  const float pb = a.post_b ? to_f32<TW>(((const TW*)a.post_b)[c]) : 0.f;
-  const float s = a.scale ? to_f32<TW>(((const TW*)a.scale)[c]) : 1.f;
+  for (int q = 0; q < kNormSums; ++q) got[q] = (float)sh[q][0][lc];
+  auto put = [&](void* p, float v) {
+    if (!p) return;
+    if (wb) ((bf16_t*)p)[c] = f32_to_bf16(v);
+    else ((float*)p)[c] = v;
+  };
+  Gate g = {1.f, 0.f};
+  if (a.gate_mode == GNNEA_GATE_ROW) g = gate_of(gate);
+  // the rows' sums are over dx times an element's own gate; a shared gate comes in here
   const float both = fmaf(pw, got[0], pb * got[1]);
-  if (a.dpost_w) ((TW*)a.dpost_w)[c] = from_f32<TW>(a.alpha * s * got[0]);
-  if (a.dpost_b) ((TW*)a.dpost_b)[c] = from_f32<TW>(a.alpha * s * got[1]);
-  if (a.dscale) ((TW*)a.dscale)[c] = from_f32<TW>(a.alpha * both);
-  if (a.dpre_w) ((TW*)a.dpre_w)[c] = from_f32<TW>(got[2]);
-  if (a.dpre_b) ((TW*)a.dpre_b)[c] = from_f32<TW>(got[3]);
-  if (a.gate_mode == GNNEA_GATE_ROW && a.dgate) {
-    const float rest = gate_of(to_f32<TW>(((const TW*)a.gate)[c])).rest;
-    ((TW*)a.dgate)[c] = from_f32<TW>(a.alpha * s * rest * both);
-  }
+  put(a.dpost_w, scale * g.g * got[0]);
+  put(a.dpost_b, scale * g.g * got[1]);
+  put(a.dscale, a.alpha * g.g * both);
+  put(a.dpre_w, got[2]);
+  put(a.dpre_b, got[3]);
+  if (a.gate_mode == GNNEA_GATE_ROW) put(a.dgate, scale * g.g * g.rest * both);
 }
 
-struct NormPlan { int tpr, nit, blocks; };
+struct NormPlan { int tpr, nit, threads, blocks; };
 
-// Threads per row: 16 lanes up to 16 chunks, a wave up to 1024 values, then the smallest workgroup
-// whose threads hold 16 values each.
+// Threads per row: 16 lanes up to 16 chunks, a wave up to 512 values, then as many waves as leave 8
+// values to a thread (the backward's twelve arrays of them fill its registers).
 static NormPlan norm_plan(int64_t n, int D, int V, bool bwd) {
-  const int chunks = (D + V - 1) / V, most = 16 / V;
+  const int chunks = (D + V - 1) / V, most = 8 / V;
   NormPlan p;
-  p.tpr = chunks <= 16 ? 16 : 64;
-  if (chunks > 64 * most) p.tpr = chunks <= 256 * most ? 256 : 512;
-  p.nit = (chunks + p.tpr - 1) / p.tpr;
-  if (p.nit == 3) p.nit = 4;
-  const int rpb = p.tpr < 256 ? 256 / p.tpr : 1;
-  const int64_t want = (n + rpb - 1) / rpb;
-  // backward: rows per workgroup go up with n, so that the column sums stay few
-  const int64_t cap = bwd ? (p.tpr >= 256 ? 256 * (1024 / p.tpr) : 256 * 4) : 256 * 32;
+  p.threads = 256;
+  if (chunks <= 64 * most) {
+    p.tpr = chunks <= 16 ? 16 : 64;
+    p.nit = (chunks + p.tpr - 1) / p.tpr;
+  } else {
+    p.nit = most;
+    p.threads = ((chunks + most - 1) / most + 63) / 64 * 64;
+    p.tpr = p.threads <= 256 ? 256 : p.threads <= 512 ? 512 : 1024;
+  }
+  const int rpb = p.tpr < 256 ? 256 / p.tpr : 1, waves = p.threads / 64;
+  // (backward: two rows at least, so that the column sums stay few)
+  const int64_t want = bwd ? (n + 2 * rpb - 1) / (2 * rpb) : (n + rpb - 1) / rpb;
+  // rows per workgroup go up with n: the workgroups fill the chip once, and each reads its next
+  // row while it computes one
+  const int fit = bwd ? (waves <= 4 ? 2 : 1) : waves <= 5 ? 4 : waves <= 10 ? 2 : 1;
+  const int64_t cap = 256 * fit;
   p.blocks = (int)(want < cap ? want : cap);
   return p;
 }
@@ -452,30 +586,42 @@ static int norm_sums(const gnnea_norm& a) {
   return s;
 }
 
-#define GNNEA_NORM_LAUNCH(K, TPR, NIT)                                                     \
-  hipLaunchKernelGGL((K<T, TW, TPR, NIT>), dim3(p.blocks), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
+template <typename T, int TPR, int NIT, bool BWD>
+static void norm_launch(const gnnea_norm& a, const NormPlan& p, hipStream_t s) {
+  const dim3 g(p.blocks), b(p.threads);
+  // (a workgroup's four sums, 16 B a value, or one sum of its rows)
+  const int lds = p.threads * NIT * RowChunk<T>::V * 4 * (TPR > 64 ? kNormSums : 1);
+  const int in = !a.y ? 0 : a.gate_mode == GNNEA_GATE_FULL ? 2 : 1;
+  if constexpr (!BWD) {
+    if (in == 0) hipLaunchKernelGGL((k_norm_fwd<T, TPR, NIT, 0>), g, b, 0, s, a);
+    else if (in == 1) hipLaunchKernelGGL((k_norm_fwd<T, TPR, NIT, 1>), g, b, 0, s, a);
+    else hipLaunchKernelGGL((k_norm_fwd<T, TPR, NIT, 2>), g, b, 0, s, a);
+  } else if (a.post_b || (a.sums & 10)) {
+    if (in == 0) hipLaunchKernelGGL((k_norm_bwd<T, TPR, NIT, 0, true>), g, b, lds, s, a);
+    else if (in == 1) hipLaunchKernelGGL((k_norm_bwd<T, TPR, NIT, 1, true>), g, b, lds, s, a);
+    else hipLaunchKernelGGL((k_norm_bwd<T, TPR, NIT, 2, true>), g, b, lds, s, a);
+  } else {
+    if (in == 0) hipLaunchKernelGGL((k_norm_bwd<T, TPR, NIT, 0, false>), g, b, lds, s, a);
+    else if (in == 1) hipLaunchKernelGGL((k_norm_bwd<T, TPR, NIT, 1, false>), g, b, lds, s, a);
+    else hipLaunchKernelGGL((k_norm_bwd<T, TPR, NIT, 2, false>), g, b, lds, s, a);
+  }
+}
 
-template <typename T, typename TW, bool BWD>
-static int norm_launch(const gnnea_norm& a, const NormPlan& p, hipStream_t s) {
+template <typename T, bool BWD>
+static int norm_shape(const gnnea_norm& a, const NormPlan& p, hipStream_t s) {
   bool done = false;
-#define GNNEA_NORM_CASE(TPR, NIT)                               \
-  if (p.tpr == TPR && p.nit == NIT) {                           \
-    if constexpr (BWD) GNNEA_NORM_LAUNCH(k_norm_bwd, TPR, NIT); \
-    else GNNEA_NORM_LAUNCH(k_norm_fwd, TPR, NIT);               \
-    done = true;                                                \
+#define GNNEA_NORM_CASE(TPR, NIT)                 \
+  if (p.tpr == TPR && p.nit == NIT) {             \
+    norm_launch<T, TPR, NIT, BWD>(a, p, s);      \
+    done = true;                                  \
   }
   GNNEA_NORM_CASE(16, 1)
   GNNEA_NORM_CASE(64, 1)
-  GNNEA_NORM_CASE(64, 2)
-  GNNEA_NORM_CASE(256, 2)
-  GNNEA_NORM_CASE(512, 2)
-  if constexpr (RowChunk<T>::V == 8) {
-    GNNEA_NORM_CASE(256, 1)
-  } else {
-    GNNEA_NORM_CASE(64, 4)
-    GNNEA_NORM_CASE(256, 4)
-    GNNEA_NORM_CASE(512, 4)
-  }
+  constexpr int M = 8 / RowChunk<T>::V;
+  if constexpr (M > 1) GNNEA_NORM_CASE(64, M)
+  GNNEA_NORM_CASE(256, M)
+  GNNEA_NORM_CASE(512, M)
+  GNNEA_NORM_CASE(1024, M)
 #undef GNNEA_NORM_CASE
   GNNEA_LAUNCH_CHECK();
   return done ? 0 : GNNEA_EINVAL;
@@ -483,9 +629,8 @@ static int norm_launch(const gnnea_norm& a, const NormPlan& p, hipStream_t s) {
 
 template <bool BWD>
 static int norm_dispatch(const gnnea_norm& a, const NormPlan& p, hipStream_t s) {
-  if (a.dtype == GNNEA_F32) return norm_launch<float, float, BWD>(a, p, s);
-  if (a.w_dtype == GNNEA_F32) return norm_launch<bf16_t, float, BWD>(a, p, s);
-  return norm_launch<bf16_t, bf16_t, BWD>(a, p, s);
+  if (a.dtype == GNNEA_F32) return norm_shape<float, BWD>(a, p, s);
+  return norm_shape<bf16_t, BWD>(a, p, s);
 }
 
 }  // namespace gnnea
@@ -523,11 +668,7 @@ extern "C" int gnnea_norm_bwd(const gnnea_norm* arg, void* ws, int64_t ws_bytes,
     if (rc2) return rc2;
   }
   if (a.sums) {  // also for no rows: the gradients are then zero
-    const int g = div_up(a.D, 64);
-    if (a.w_dtype == GNNEA_F32)
-      hipLaunchKernelGGL(k_norm_fold<float>, dim3(g), dim3(1024), 0, s, a, p.blocks);
-    else
-      hipLaunchKernelGGL(k_norm_fold<bf16_t>, dim3(g), dim3(1024), 0, s, a, p.blocks);
+    hipLaunchKernelGGL(k_norm_fold, dim3(div_up(a.D, 16)), dim3(1024), 0, s, a, p.blocks);
     GNNEA_LAUNCH_CHECK();
   }
   return 0;

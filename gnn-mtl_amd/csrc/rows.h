@@ -11,12 +11,15 @@ template <> struct RowChunk<bf16_t> { static constexpr int V = 8; };
 
 // 16 bytes at the alignment of one element: global memory takes them at any address, so a row of
 // an odd width costs no narrower accesses
-template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Raw16 { uint32_t w[4]; };
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename T> struct Raw16;
+template <> struct Raw16<float> { typedef u32x4 type __attribute__((aligned(4))); };
+template <> struct Raw16<bf16_t> { typedef u32x4 type __attribute__((aligned(2))); };
 
 template <typename T>
 __device__ __forceinline__ uint4 load16(const T* p) {
-  const Raw16<T> r = *(const Raw16<T>*)p;
-  return make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+  const u32x4 r = *(const typename Raw16<T>::type*)p;
+  return make_uint4(r.x, r.y, r.z, r.w);
 }
 
 // `left` elements (at most V) from p, zeros after them
@@ -33,16 +36,13 @@ __device__ __forceinline__ void load_chunk(const T* p, int left, float (&f)[V]) 
 template <typename T, int V>
 __device__ __forceinline__ void store_chunk(T* p, int left, const float (&f)[V]) {
   if (left >= V) {
-    Raw16<T> r;
-    if constexpr (V == 4) {
+    u32x4 r;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) r.w[k] = __builtin_bit_cast(uint32_t, f[k]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        r.w[k] = (uint32_t)f32_to_bf16(f[2 * k]) | ((uint32_t)f32_to_bf16(f[2 * k + 1]) << 16);
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (V == 4) r[k] = __builtin_bit_cast(uint32_t, f[k]);
+      else r[k] = x3_cvt2(x3_f32x2{f[2 * k], f[2 * k + 1]});
     }
-    *(Raw16<T>*)p = r;
+    *(typename Raw16<T>::type*)p = r;
   } else {
 #pragma unroll
     for (int k = 0; k < V; ++k)

@@ -153,4 +153,7 @@ def dot_attention(adj, q, k, v, heads, kv_heads=None, scale=None):
         raise ValueError("gnnea.dot_attention: d_head must be at most %d (got %d)"
                          % (MAX_D_HEAD, d))
     scale = d ** -0.5 if scale is None else float(scale)
-    return DotAttentionFn.apply(_rows(q), _rows(k), _rows(v), csr, (heads, kv_heads, scale))
+    k, v = _rows(k), _rows(v)
+    if _ld(k) != _ld(v):  # the kernels form one row offset for both
+        k, v = k.contiguous(), v.contiguous()
+    return DotAttentionFn.apply(_rows(q), k, v, csr, (heads, kv_heads, scale))

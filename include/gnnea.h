@@ -940,13 +940,13 @@ int gnnea_adamw_moments(const gnnea_adamw_tensor* tensors, int32_t count, void* 
  * layers/att_layers.py:29-61): for row i and head h, with key/value head j = h / (heads / kv_heads),
  *   o_i = sum_c p_ic v_c,   p_ic = softmax over the row's entries c of (scale q_i . k_c)
  * q, o: n_rows x heads d_head; k, v: n_cols x kv_heads d_head (type GNNEA_F32 or GNNEA_BF16, row
- * strides in elements, any alignment of an element); lse: n_rows x heads floats, the log of the
- * row's sum of exponentials; a row without entries gives o = 0 and lse = -inf.  k and v of columns
+ * strides in elements, any alignment of an element); lse: n_rows x heads floats, the base-2
+ * logarithm of the row's sum of exponentials; the row passes need ldk == ldv; a row without entries gives o = 0 and lse = -inf.  k and v of columns
  * that no row has stored are never read.  heads % kv_heads == 0, d_head <= 256.  The matrix's
  * values are not used.
- * Backward, the probabilities recomputed as p = exp(scale q.k - lse), dp = do . v:
+ * Backward, the probabilities recomputed from the scores and lse, dp = do . v:
  *   _bwd_rows  dq_i = scale (sum p dp k - delta sum p k), delta_i = sum p dp, over the matrix's
- *              rows; writes stat: n_rows x heads x {lse in powers of two, delta} floats
+ *              rows; writes stat: n_rows x heads x {lse, delta} floats
  *   _bwd_cols  dk, dv (summed over the heads that share a key/value head) over the transposed
  *              matrix's rows; reads stat
  * Rows of dq, dk, dv without entries are written with zeros.  Sums are fp32 in a fixed order.
