@@ -71,7 +71,7 @@ class NormFn(torch.autograd.Function):
             with _lib.on_device(x.device):
                 check(_lib.lib().gnnea_norm_fwd(a, stream_of(x.device)))
         ctx.save_for_backward(x, y, gate, scale, pw, pb, qw, qb, stats)
-        ctx.meta = meta
+        ctx.problem = a  # (the addresses of the saved tensors; the backward adds its own to a copy)
         ctx.set_materialize_grads(False)
         return r, h
 
@@ -86,8 +86,7 @@ class NormFn(torch.autograd.Function):
         if n == 0:
             return tuple(torch.zeros_like(t) if t is not None and need else None for t, need in
                          zip((x, y, gate) + vecs + (None,), ctx.needs_input_grad))
-        a = _problem(x, y, gate, vecs, ctx.meta)
-        a.stats = stats.data_ptr()
+        a = NormProblem.from_buffer_copy(ctx.problem)
         if dr is not None:
             dr = _rows(dr, x.dtype)
             a.dr, a.lddr = dr.data_ptr(), _ld(dr)

@@ -5,10 +5,11 @@ the same loop (``weight_decay=0`` is Adam), with the gradients' global norm clip
 step where ``max_norm`` is given.  The step counter and the learning rate stay on the device, so a
 step can be captured into a HIP graph as it is.
 """
+import numpy as np
 import torch
 
 from . import _lib
-from ._lib import AdamwTensor, check, ptr, stream_of
+from ._lib import check, ptr, stream_of
 from .ops import FEATURE_DTYPES
 
 BLOCK = _lib.GNNEA_ADAMW_BLOCK
@@ -58,17 +59,17 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.max_norm = state_bits, max_norm
         self.seed = int(seed) & 0xffffffff
         self.grad_norm = None
-        self._index = {}  # parameter -> its number in the hash of the 8-bit rounding
+        self._base = []  # number of a group's first parameter in the hash of the 8-bit rounding
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, group):
+        self._base.append(sum(len(g["params"]) for g in self.param_groups))
         super().add_param_group(group)
         for p in self.param_groups[-1]["params"]:
             if p.dtype not in FEATURE_DTYPES:
                 raise TypeError("gnnea.AdamW: fp32 or bf16 parameters required (got %s)" % p.dtype)
             if p.is_sparse or not _dense(p):
                 raise ValueError("gnnea.AdamW: parameters must be dense and without gaps")
-            self._index[p] = len(self._index)
 
     def _init_state(self, p, step):
         if torch.cuda.is_current_stream_capturing():
@@ -86,23 +87,21 @@ class AdamW(torch.optim.Optimizer):
             # the exponents of m's and of sqrt(v)'s blocks (any valid one: every code is zero)
             s["scales"] = torch.full((2, -(-n // BLOCK)), 127, dtype=torch.uint8, device=p.device)
 
-    def _tensor(self, t, p, g):
-        s = self.state[p]
-        t.p, t.g, t.m, t.n = p.data_ptr(), g, s["exp_avg"].data_ptr(), p.numel()
+    def _state_row(self, s):
+        """m, the second moment, the scales and the length of a state, for a descriptor."""
+        m = s["exp_avg"]
         if self.state_bits == 32:
-            t.v = s["exp_avg_sq"].data_ptr()
-        else:
-            t.v, t.scales = s["exp_avg_rms"].data_ptr(), s["scales"].data_ptr()
-        t.index = self._index[p]
+            return (m.data_ptr(), s["exp_avg_sq"].data_ptr(), 0, m.numel())
+        return (m.data_ptr(), s["exp_avg_rms"].data_ptr(), s["scales"].data_ptr(), m.numel())
 
     @staticmethod
-    def _gradient(p):
-        g = p.grad
-        if g.is_sparse or g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
+    def _gradient(p, g, n):
+        """g with p's order of elements (torch has seen to it that shapes and devices agree)."""
+        if g.is_sparse or g.dtype != p.dtype or g.numel() != n or p.numel() != n:
             raise ValueError("gnnea.AdamW: gradients must be dense and like their parameter")
-        if g.stride() != p.stride():  # the same order of elements as the parameter
-            g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
-        return g
+        if (g.is_contiguous() and p.is_contiguous()) or g.stride() == p.stride():
+            return g
+        return torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -110,32 +109,46 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        groups, held = [], []
-        device = None
-        for group in self.param_groups:
-            ps = [p for p in group["params"] if p.grad is not None]
-            if not ps:
+        groups, held, device = [], [], None
+        state = self.state
+        for base, group in zip(self._base, self.param_groups):
+            lists, step, fresh = {}, None, []
+            for i, p in enumerate(group["params"]):
+                s = state.get(p)
+                if s is not None and step is None:
+                    step = s["step"]
+                g = p.grad
+                if g is None:
+                    continue
+                if device is None:
+                    _lib.require_device(p)
+                    device = p.device
+                if s is None:
+                    fresh.append((i, p, g))
+                    continue
+                row = self._state_row(s)
+                g = self._gradient(p, g, row[3])
+                held.append(g)
+                lists.setdefault(p.dtype, []).append((p.data_ptr(), g.data_ptr()) + row
+                                                     + (base + i,))
+            for i, p, g in fresh:
+                if p.device != device:
+                    raise ValueError("gnnea.AdamW: parameters on more than one device")
+                if step is None:
+                    step = torch.zeros(1, dtype=torch.int64, device=device)
+                g = self._gradient(p, g, p.numel())
+                held.append(g)
+                self._init_state(p, step)
+                lists.setdefault(p.dtype, []).append((p.data_ptr(), g.data_ptr())
+                                                     + self._state_row(state[p]) + (base + i,))
+            if not lists:
                 continue
-            _lib.require_device(*ps)
-            device = device or ps[0].device
-            if any(p.device != device for p in ps):
-                raise ValueError("gnnea.AdamW: parameters on more than one device")
-            steps = [self.state[p]["step"] for p in group["params"] if p in self.state]
-            step = steps[0] if steps else torch.zeros(1, dtype=torch.int64, device=device)
-            lists = {}
-            for p in ps:
-                if p not in self.state:
-                    self._init_state(p, step)
-                lists.setdefault(p.dtype, []).append(p)
             arrays = []
-            for dtype, those in lists.items():
-                arr = (AdamwTensor * len(those))()
-                for t, p in zip(arr, those):
-                    g = self._gradient(p)
-                    held.append(g)
-                    self._tensor(t, p, g.data_ptr())
-                arrays.append((arr, len(those), _lib.GNNEA_BF16 if dtype == torch.bfloat16
-                               else _lib.GNNEA_F32))
+            for dtype, rows in lists.items():
+                table = np.array(rows, dtype=np.int64)
+                held.append(table)
+                arrays.append((table.ctypes.data, len(rows), _lib.GNNEA_BF16
+                               if dtype == torch.bfloat16 else _lib.GNNEA_F32))
             groups.append((group, step, arrays))
         if not groups:
             return loss
@@ -174,25 +187,25 @@ class AdamW(torch.optim.Optimizer):
         """[(m, second)] of all parameters in order, (None, None) before their first step: with
         32 bits the state's own exp_avg and exp_avg_sq; with 8 bits what the codes of m and of
         sqrt(v) stand for, exactly, in bf16 tensors of the parameter's shape."""
-        ps = [p for group in self.param_groups for p in group["params"]]
-        if self.state_bits == 32:
-            return [(self.state[p]["exp_avg"], self.state[p]["exp_avg_sq"]) if p in self.state
-                    else (None, None) for p in ps]
-        out, have = [], [p for p in ps if p in self.state]
-        arr = (AdamwTensor * max(len(have), 1))()
-        at = 0
-        for p in ps:
-            if p not in self.state:
-                out.append((None, None))
-                continue
-            m, u = (torch.empty_like(p, dtype=torch.bfloat16) for _ in range(2))
-            self._tensor(arr[at], p, u.data_ptr())
-            arr[at].p = m.data_ptr()
-            at += 1
-            out.append((m, u))
-        if have:
-            with _lib.on_device(have[0].device):
-                check(_lib.lib().gnnea_adamw_moments(arr, at, stream_of(have[0].device)))
+        state, out, rows = self.state, [], []
+        for group in self.param_groups:
+            for p in group["params"]:
+                s = state.get(p)
+                if s is None:
+                    out.append((None, None))
+                elif self.state_bits == 32:
+                    out.append((s["exp_avg"], s["exp_avg_sq"]))
+                else:
+                    m = torch.empty_like(p, dtype=torch.bfloat16)
+                    u = torch.empty_like(p, dtype=torch.bfloat16)
+                    rows.append((m.data_ptr(), u.data_ptr()) + self._state_row(s) + (0,))
+                    out.append((m, u))
+        if rows:
+            device = next(m.device for m, _ in out if m is not None)
+            table = np.array(rows, dtype=np.int64)
+            with _lib.on_device(device):
+                check(_lib.lib().gnnea_adamw_moments(table.ctypes.data, len(rows),
+                                                     stream_of(device)))
         return out
 
     def load_state_dict(self, state_dict):
