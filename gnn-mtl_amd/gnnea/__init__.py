@@ -1,7 +1,8 @@
 """gnnea — MI355X-native hot path of the GNN entity-alignment engine.
 
 Host package around libgnnea.so (include/gnnea.h): device CSR cache (graph), HIP ops and their
-autograd wrappers (ops), the Sinkhorn host driver (sinkhorn), synthetic inputs (synth) and the
+autograd wrappers (ops), dot-product attention over an adjacency (attention), residual norms (norm),
+AdamW (optim), the Sinkhorn host driver (sinkhorn), synthetic inputs (synth) and the
 multi-GPU node sharding (dist).  The drop-in mirrors of the reference modules live next to this
 package (layers/, models/, utils/, SinkhornOT/) and call into it.
 """

@@ -399,6 +399,14 @@ class DistAdj:
                                           _lib.GNNEA_ACT_IDENTITY))
         return HaloGATFn.apply(H, a_all, self, heads, d_head, alpha, code)
 
+    def dot_attention(self, q, k, v, heads, kv_heads=None):
+        """Dot-product attention of the shard's rows (gnnea.attention); one rank per KG group."""
+        csr = self.local_csr()
+        if csr is None:
+            raise NotImplementedError("gnnea: dot-product attention on a row-sharded adjacency")
+        from .attention import dot_attention
+        return dot_attention(csr, q, k, v, heads, kv_heads)
+
     def highway_fwd(self, hidden, gate_pre, resid, bias_gate, act):
         """HighWay tail over the shard (gnnea.ops.HighwayLayerFn's aggregation hook): the
         group's hidden rows by the halo all-gather, gate_pre / resid row-local."""

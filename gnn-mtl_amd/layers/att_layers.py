@@ -13,6 +13,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from gnnea import ops
+from gnnea.attention import dot_attention
 from gnnea.dist_graph import DistAdj
 from gnnea.graph import csr_of, dense_of
 
@@ -100,3 +101,41 @@ class GraphAttentionLayer(nn.Module):
             y = ops.head_mean(y, heads, self.output_dim)
         y = F.dropout(y, self.dropout, training=self.training)
         return (y, adj)
+
+
+class DotAttentionLayer(nn.Module):
+    """Multi-head dot-product attention over the adjacency, forward((x, adj)) -> (h, adj) like
+    GraphAttentionLayer: h = act(softmax_j(q_i . k_j / sqrt(d)) v), heads concatenated or averaged.
+    q, k and v are columns of one projection W; ``kv_heads`` key/value heads (None: nheads) are
+    shared by groups of query heads.  The adjacency's values are not used; a node without stored
+    entries gets act(0)."""
+
+    def __init__(self, input_dim, output_dim, dropout, activation, nheads, concat, kv_heads=None):
+        super(DotAttentionLayer, self).__init__()
+        kv_heads = nheads if kv_heads is None else kv_heads
+        if nheads % kv_heads:
+            raise ValueError("gnnea: nheads must be a multiple of kv_heads (got %d, %d)"
+                             % (nheads, kv_heads))
+        self.dropout, self.output_dim, self.concat = dropout, output_dim, concat
+        self.nheads, self.kv_heads, self.act = nheads, kv_heads, activation
+        self.W = nn.Parameter(torch.zeros(size=(input_dim, (nheads + 2 * kv_heads) * output_dim)))
+        nn.init.xavier_normal_(self.W.data, gain=1.414)
+
+    def forward(self, input):
+        x, adj = input
+        x = F.dropout(dense_of(x), self.dropout, training=self.training)
+        qkv = ops.matmul(x, self.W)
+        wq, wk = self.nheads * self.output_dim, self.kv_heads * self.output_dim
+        q, k, v = qkv[:, :wq], qkv[:, wq:wq + wk], qkv[:, wq + wk:]
+        if isinstance(adj, DistAdj):
+            y = adj.dot_attention(q, k, v, self.nheads, self.kv_heads)
+        else:
+            y = dot_attention(adj, q, k, v, self.nheads, self.kv_heads)
+        if not self.concat:
+            y = ops.head_mean(y, self.nheads, self.output_dim)
+        y = F.dropout(self.act(y), self.dropout, training=self.training)
+        return (y, adj)
+
+    def extra_repr(self):
+        return 'heads={}, kv_heads={}, head_dim={}'.format(self.nheads, self.kv_heads,
+                                                           self.output_dim)

@@ -17,7 +17,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.nn.modules.module import Module
 
-from gnnea import _lib, ops
+from gnnea import _lib, norm, ops
 from gnnea.dist_graph import DistAdj
 from gnnea.graph import dense_of
 
@@ -128,3 +128,44 @@ class Linear(Module):
             return F.dropout(h, self.dropout, training=self.training)
         h = ops.linear(dense_of(x), self.linear.weight, self.linear.bias)
         return self.act(F.dropout(h, self.dropout, training=self.training))
+
+
+class ResidualStack(Module):
+    """Layers of one width as residual blocks with norms before and after each (gnnea.norm):
+
+        h_0 = N(x);   y_i = layer_i(h_i);   x = x + scale_i * sigmoid(gate_i) * N_i(y_i);
+        h_{i+1} = N'_i(x)
+
+    forward((x, adj)) -> (h_last, adj).  ``kind``: "rms" or "layer" (with biases); ``gate``: a
+    learned gate per feature and block; ``scale``: where the learned residual scales start."""
+
+    def __init__(self, layers, dim, kind="rms", gate=False, scale=1.0):
+        super(ResidualStack, self).__init__()
+        if kind not in norm.KINDS:
+            raise ValueError("gnnea: kind must be 'rms' or 'layer' (got %r)" % (kind,))
+        self.blocks = nn.ModuleList(layers)
+        self.kind = kind
+        n, bias = len(self.blocks), kind == "layer"
+
+        def vectors(count, value, want=True):
+            return nn.ParameterList([nn.Parameter(torch.full((dim,), float(value)))
+                                     for _ in range(count if want else 0)])
+        self.pre_weight, self.pre_bias = vectors(n + 1, 1), vectors(n + 1, 0, bias)
+        self.post_weight, self.post_bias = vectors(n, 1), vectors(n, 0, bias)
+        self.scale, self.gate = vectors(n, scale), vectors(n, 0, gate)
+
+    def forward(self, input):
+        x, adj = input
+        x = dense_of(x)
+
+        def at(vectors, i):
+            return vectors[i] if len(vectors) else None
+        h = norm.norm(x, self.pre_weight[0], at(self.pre_bias, 0), kind=self.kind)
+        for i, block in enumerate(self.blocks):
+            y, _ = block((h, adj))
+            x, h = norm.residual_norm(
+                x, y, gate=at(self.gate, i), scale=self.scale[i],
+                post_weight=self.post_weight[i], post_bias=at(self.post_bias, i),
+                pre_weight=self.pre_weight[i + 1], pre_bias=at(self.pre_bias, i + 1),
+                kind=self.kind)
+        return h, adj

@@ -2,11 +2,17 @@
 
 Each encoder stacks ``num_layers - 1`` layers in an ``nn.Sequential`` called ``layers`` (so the
 state_dict keys are ``layers.{i}....`` as in the reference) and exposes ``encode(x, adj)``.
+
+Beyond the reference: ``args.residual`` ("rms" or "layer") stacks the graph layers as residual
+blocks with norms (layers.layers.ResidualStack; feat_dim must equal dim; ``args.residual_gate``
+adds gates), and ``args.attention = "dot"`` gives GAT dot-product attention with
+``args.kv_heads`` key/value heads (layers.att_layers.DotAttentionLayer).
 """
 import torch.nn as nn
 
-from layers.att_layers import GraphAttentionLayer
-from layers.layers import GraphConvolution, HighWayGraphConvolution, Linear, get_dim_act
+from layers.att_layers import DotAttentionLayer, GraphAttentionLayer
+from layers.layers import (GraphConvolution, HighWayGraphConvolution, Linear, ResidualStack,
+                           get_dim_act)
 
 
 class Encoder(nn.Module):
@@ -21,11 +27,16 @@ class Encoder(nn.Module):
         return out
 
 
-def _stack(args, make):
+def _stack(args, make, graph=True):
     assert args.num_layers > 0
     dims, acts = get_dim_act(args)
-    return nn.Sequential(*[make(d_in, d_out, act)
-                           for d_in, d_out, act in zip(dims[:-1], dims[1:], acts)])
+    layers = [make(d_in, d_out, act) for d_in, d_out, act in zip(dims[:-1], dims[1:], acts)]
+    kind = getattr(args, "residual", None)
+    if not kind or not graph:
+        return nn.Sequential(*layers)
+    if len(set(dims)) != 1:
+        raise ValueError("gnnea: residual blocks need feat_dim == dim (got %s)" % (dims,))
+    return ResidualStack(layers, dims[0], kind, bool(getattr(args, "residual_gate", False)))
 
 
 class MLP(Encoder):
@@ -33,7 +44,8 @@ class MLP(Encoder):
 
     def __init__(self, args):
         super(MLP, self).__init__()
-        self.layers = _stack(args, lambda i, o, act: Linear(i, o, args.dropout, act, args.bias))
+        self.layers = _stack(args, lambda i, o, act: Linear(i, o, args.dropout, act, args.bias),
+                             graph=False)
         self.encode_graph = False
 
 
@@ -60,6 +72,9 @@ class GAT(Encoder):
 
         def make(i, o, act):
             assert o % args.n_heads == 0
+            if getattr(args, "attention", "additive") == "dot":
+                return DotAttentionLayer(i, o // args.n_heads, args.dropout, act, args.n_heads,
+                                         True, getattr(args, "kv_heads", None))
             return GraphAttentionLayer(i, o // args.n_heads, args.dropout, act, args.alpha,
                                        args.n_heads, True)
 

@@ -150,3 +150,36 @@ def test_host_tensors_are_refused():
     p.grad = x
     with pytest.raises(GnneaError):
         AdamW([p]).step()
+
+
+def encoder_args(**kw):
+    import types
+    a = dict(num_layers=3, dim=12, feat_dim=12, act="relu", dropout=0.0, bias=1, n_heads=4,
+             alpha=0.2, cuda=-1, device="cpu")
+    a.update(kw)
+    return types.SimpleNamespace(**a)
+
+
+def test_encoder_options():
+    """Without the options the encoders are what they were; with them, residual stacks and
+    dot-product layers with parameters of these names and shapes."""
+    from layers.att_layers import DotAttentionLayer
+    from layers.layers import ResidualStack
+    from models.encoders import GAT, GCN, HGCN, MLP
+    for cls in (GCN, GAT, HGCN, MLP):
+        assert isinstance(cls(encoder_args()).layers, torch.nn.Sequential)
+    assert isinstance(MLP(encoder_args(residual="rms")).layers, torch.nn.Sequential)
+    enc = GAT(encoder_args(attention="dot", kv_heads=2, residual="layer", residual_gate=True))
+    assert isinstance(enc.layers, ResidualStack)
+    assert isinstance(enc.layers.blocks[0], DotAttentionLayer)
+    sd = enc.state_dict()
+    assert sd["layers.blocks.1.W"].shape == (12, (4 + 2 * 2) * 3)
+    assert {"layers.pre_weight.2", "layers.pre_bias.2", "layers.post_weight.1", "layers.post_bias.1",
+            "layers.scale.1", "layers.gate.1"} <= set(sd)
+    assert "layers.gate.0" not in GCN(encoder_args(residual="rms")).state_dict()
+    with pytest.raises(ValueError):
+        GCN(encoder_args(residual="rms", feat_dim=10))
+    with pytest.raises(ValueError):
+        GCN(encoder_args(residual="batch"))
+    with pytest.raises(ValueError):
+        DotAttentionLayer(12, 3, 0.0, torch.relu, 4, True, kv_heads=3)

@@ -11,6 +11,10 @@ same, so the difference is expected to be exactly zero), then times eager steps 
 (HIP events, median).
 
     python tools/graph_step.py [--model GCN|HGCN|GAT] [--entities 15000] [--steps 50]
+        [--optim adam|adamw|adamw8] [--attention dot] [--residual rms|layer]
+
+--optim adamw / adamw8: gnnea.optim.AdamW with 32- or 8-bit moments and gradients clipped to norm 1
+instead of torch's Adam; --attention and --residual: the encoders' options of these names.
 """
 import argparse
 import json
@@ -30,13 +34,13 @@ from gnnea.margin import margin_loss  # noqa: E402
 from tools.dist_step import loss_indices  # noqa: E402
 
 
-def build(model, n, t, dev, seed=10086):
+def build(model, n, t, dev, seed=10086, **options):
     import types
     from models.decoders import model2decoder
     from models.encoders import model2encoder
     a = types.SimpleNamespace(model=model, num_layers=3, dim=300, act="relu", dropout=0.0,
                               bias=1, n_heads=4, alpha=0.2, feat_dim=300, n_classes=300,
-                              cuda=0, device=dev)
+                              cuda=0, device=dev, **options)
     torch.manual_seed(seed)
     enc = model2encoder[model](a).to(dev)
     dec = model2decoder[model](a).to(dev)
@@ -67,15 +71,23 @@ def median_ms(fn, reps):
     return float(np.median([a.elapsed_time(b) for a, b in evs]))
 
 
-def run(model, n, t, steps, dev):
-    enc, dec, dadj = build(model, n, t, dev)
+def optimizer(params, optim):
+    if optim == "adam":
+        # (capturable: the step counter and the bias corrections stay on the device)
+        return torch.optim.Adam(params, lr=0.005, capturable=True)
+    from gnnea.optim import AdamW
+    return AdamW(params, lr=0.005, weight_decay=0.0, state_bits=8 if optim == "adamw8" else 32,
+                 max_norm=1.0)
+
+
+def run(model, n, t, steps, dev, optim="adam", **options):
+    enc, dec, dadj = build(model, n, t, dev, **options)
     g = torch.Generator(device=dev).manual_seed(1)
     x = torch.randn(2 * n, 300, device=dev, generator=g)
     x /= x.norm(dim=1, keepdim=True)
     idx, t_, k_ = loss_indices(n)
     params = list(enc.parameters()) + list(dec.parameters())
-    # (capturable: the step counter and the bias corrections stay on the device)
-    opt = torch.optim.Adam(params, lr=0.005, capturable=True)
+    opt = optimizer(params, optim)
 
     def step():
         out = dec.decode(enc.encode(x, dadj), dadj)
@@ -144,7 +156,8 @@ def run(model, n, t, steps, dev):
     graph_wall = wall_ms(replay, steps)
     return {"model": model + "-EA", "graph": "2x%d entities, %d triples per KG, %d nnz"
             % (n, t, dadj.nnz), "step": "encode + decode + margin loss (t=%d, k=%d) + backward "
-            "+ Adam (capturable)" % (t_, k_), "steps": steps,
+            "+ %s" % (t_, k_, "Adam (capturable)" if optim == "adam" else optim),
+            "steps": steps,
             "eager_ms": round(eager_ms, 4), "graph_ms": round(graph_ms, 4),
             "speedup": round(eager_ms / graph_ms, 3),
             "eager_wall_ms": round(eager_wall, 4), "graph_wall_ms": round(graph_wall, 4),
@@ -159,11 +172,15 @@ def main():
     ap.add_argument("--entities", type=int, default=synth.CONFIGS["dbp15k"]["n"])
     ap.add_argument("--triples", type=int, default=synth.CONFIGS["dbp15k"]["t"])
     ap.add_argument("--steps", type=int, default=50)
+    ap.add_argument("--optim", default="adam", choices=("adam", "adamw", "adamw8"))
+    ap.add_argument("--attention", default="additive", choices=("additive", "dot"))
+    ap.add_argument("--residual", default=None, choices=("rms", "layer"))
     args = ap.parse_args()
     dev = torch.device("cuda", 0)
     models = ("GCN", "HGCN", "GAT") if args.model == "all" else (args.model,)
     for m in models:
-        print(json.dumps(run(m, args.entities, args.triples, args.steps, dev)), flush=True)
+        print(json.dumps(run(m, args.entities, args.triples, args.steps, dev, args.optim,
+                             attention=args.attention, residual=args.residual)), flush=True)
 
 
 if __name__ == "__main__":
