@@ -169,16 +169,19 @@ __device__ __forceinline__ void clear(float (&f)[NCH][V]) {
 
 struct AttnUnit { int row, beg, end, slot; };
 
-// The wave's piece of a long row (these come first: they run longest), or its row (slot < 0).
-// False: nothing to do.
+// The wave's piece of a long row (their workgroups come first: they run longest), or its row (slot
+// < 0).  Consecutive rows share an XCD: neighbours in the ring of entities share keys, and rows
+// that are not whole cache lines share lines.  False: nothing to do.
 __device__ __forceinline__ bool attn_unit(const gnnea_attn& a, AttnUnit& u) {
-  int id = blockIdx.x * 4 + wave_id();
-  if (id < a.n_items) {
+  const int pb = (a.n_items + 3) / 4, b = blockIdx.x;
+  if (b < pb) {
+    const int id = b * 4 + wave_id();
+    if (id >= a.n_items) return false;
     const int4 it = ((const int4*)a.items)[id];
     u.row = it.x; u.beg = it.y; u.end = it.z; u.slot = it.w;
     return true;
   }
-  id -= a.n_items;
+  const int id = xcd_remap(b - pb, (int)gridDim.x - pb) * 4 + wave_id();
   if (id >= a.n_rows) return false;
   u.row = id; u.beg = a.rowptr[id]; u.end = a.rowptr[id + 1]; u.slot = -1;
   return a.limit == 0 || u.end - u.beg <= a.limit;
@@ -640,7 +643,7 @@ static AttnPlan attn_plan(const gnnea_attn* a, int pass) {
 template <typename T, int LPH, int NCH, bool FULL>
 static void attn_launch(const gnnea_attn& a, int pass, const AttnPlan& p, float* ws,
                         hipStream_t s) {
-  const dim3 grid(div_up((int64_t)a.n_items + a.n_rows, 4), p.units_y);
+  const dim3 grid(div_up(a.n_items, 4) + div_up(a.n_rows, 4), p.units_y);
   if (pass == GNNEA_ATTN_FWD)
     hipLaunchKernelGGL((k_attn_fwd<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, p.hpw, ws);
   else if (pass == GNNEA_ATTN_BWD_ROWS)

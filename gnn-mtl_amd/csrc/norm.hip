@@ -39,10 +39,38 @@ __device__ __forceinline__ Gate gate_of(float z) {
   return z >= 0.f ? Gate{r, e * r} : Gate{e * r, r};
 }
 
+typedef uint32_t Half4 __attribute__((ext_vector_type(2), aligned(2)));  // four bf16
+
 // value c of a vector of either type, `none` where there is none
 __device__ __forceinline__ float vec_at(const void* p, bool bf16, int c, float none) {
   if (!p) return none;
   return bf16 ? bf16_to_f32(((const bf16_t*)p)[c]) : ((const float*)p)[c];
+}
+
+// V values of a vector of either type from column c on (D: its length)
+template <int V>
+__device__ __forceinline__ void vec_chunk(const void* p, bool bf16, int c, int D, float none,
+                                          float (&f)[V]) {
+  if (!p || D < V) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = vec_at(p, bf16, c + k < D ? c + k : D - 1, none);
+  } else if (bf16) {
+#pragma unroll
+    for (int k = 0; k < V; k += 4) {
+      const Half4 r = *(const Half4*)((const bf16_t*)p + c + k);
+      const float4 v = Vec4<bf16_t>::get(make_uint2(r.x, r.y));
+      f[k] = v.x; f[k + 1] = v.y; f[k + 2] = v.z; f[k + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; k += 4) {
+      const uint4 r = load16<float>((const float*)p + c + k);
+      f[k] = __builtin_bit_cast(float, r.x);
+      f[k + 1] = __builtin_bit_cast(float, r.y);
+      f[k + 2] = __builtin_bit_cast(float, r.z);
+      f[k + 3] = __builtin_bit_cast(float, r.w);
+    }
+  }
 }
 
 // The columns of a thread: chunk i of NIT begins at column (i TPR + t) V; the last chunk of a row
@@ -191,6 +219,20 @@ __device__ __forceinline__ void wave_shares(const Cols<TPR, NIT, V>& C, float* s
   }
 }
 
+template <int NIT, int V>
+__device__ __forceinline__ void clear_row(float (&f)[NIT][V]) {
+#pragma unroll
+  for (int i = 0; i < NIT; ++i)
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[i][k] = 0.f;
+}
+
+// Where workgroup b of `blocks` leaves sum q of column c: 16 columns' four sums together, the
+// workgroups' next to each other, as they are read.
+__device__ __forceinline__ int64_t part_at(int c, int b, int blocks, int q) {
+  return (((int64_t)(c >> 4) * blocks + b) * kNormSums + q) * 16 + (c & 15);
+}
+
 // IN: 0: no y; 1: y; 2: y and a gate of its own for every element (a gate shared by all rows is
 // part of the thread's constants: P = alpha scale g post_w, Q = alpha scale g post_b)
 template <typename T, int TPR, int NIT, int IN>
@@ -204,22 +246,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const gnnea_
   __shared__ float share[16];
   wave_shares(C, share);
   float P[NIT][V], Q[NIT][V], W[NIT][V], B[NIT][V];
-#pragma unroll
-  for (int i = 0; i < NIT; ++i)
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int c = min(C.at(i) + k, a.D - 1);
-      if constexpr (IN) {
-        float s = a.alpha * vec_at(a.scale, wb, c, 1.f);
-        if (a.gate_mode == GNNEA_GATE_ROW) s *= gate_of(vec_at(a.gate, wb, c, 0.f)).g;
-        P[i][k] = s * vec_at(a.post_w, wb, c, 1.f);
-        Q[i][k] = s * vec_at(a.post_b, wb, c, 0.f);
-      }
-      W[i][k] = vec_at(a.pre_w, wb, c, 1.f);
-      B[i][k] = vec_at(a.pre_b, wb, c, 0.f);
-    }
   const int64_t step = (int64_t)gridDim.x * RPB;
-  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  int64_t row = (int64_t)xcd_remap(blockIdx.x, gridDim.x) * RPB + threadIdx.x / TPR;
   uint4 rx[NIT], ry[NIT], rz[NIT];
   auto load = [&](int64_t at) {
     load_row<T>(C, (const T*)a.x + at * a.ldx, rx);
@@ -227,6 +255,26 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const gnnea_
     if constexpr (IN == 2) load_row<T>(C, (const T*)a.gate + at * a.ldg, rz);
   };
   if (row < a.n) load(row);
+#pragma unroll
+  for (int i = 0; i < NIT; ++i) {
+    const int c = min(C.at(i), max(a.D - V, 0));  // (lanes past the row: anything that is there)
+    if constexpr (IN) {
+      float s[V], g[V];
+      vec_chunk(a.scale, wb, c, a.D, 1.f, s);
+      vec_chunk(a.post_w, wb, c, a.D, 1.f, P[i]);
+      vec_chunk(a.post_b, wb, c, a.D, 0.f, Q[i]);
+      if (a.gate_mode == GNNEA_GATE_ROW) vec_chunk(a.gate, wb, c, a.D, 0.f, g);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        s[k] *= a.alpha;
+        if (a.gate_mode == GNNEA_GATE_ROW) s[k] *= gate_of(g[k]).g;
+        P[i][k] *= s[k];
+        Q[i][k] *= s[k];
+      }
+    }
+    vec_chunk(a.pre_w, wb, c, a.D, 1.f, W[i]);
+    vec_chunk(a.pre_b, wb, c, a.D, 0.f, B[i]);
+  }
   for (; row < a.n; row += step) {
     float r[NIT][V], y[NIT][V], z[NIT][V];
 #pragma unroll
@@ -283,21 +331,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
   const bool layer = a.kind == GNNEA_NORM_LAYER, wb = a.w_dtype == GNNEA_BF16;
   const float inv = 1.f / (float)a.D;
   float P[NIT][V], Q[NIT][V], W[NIT][V], acc[kHeld][NIT][V];
+  if constexpr (!kLds) {
 #pragma unroll
-  for (int i = 0; i < NIT; ++i)
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int c = min(C.at(i) + k, a.D - 1);
-      if constexpr (IN) {
-        float s = a.alpha * vec_at(a.scale, wb, c, 1.f);
-        if (a.gate_mode == GNNEA_GATE_ROW) s *= gate_of(vec_at(a.gate, wb, c, 0.f)).g;
-        P[i][k] = s * vec_at(a.post_w, wb, c, 1.f);
-        Q[i][k] = BIAS ? s * vec_at(a.post_b, wb, c, 0.f) : 0.f;
-      }
-      W[i][k] = vec_at(a.pre_w, wb, c, 1.f);
-#pragma unroll
-      for (int q = 0; q < kHeld; ++q) acc[q][i][k] = 0.f;
-    }
+    for (int q = 0; q < kHeld; ++q) clear_row(acc[q]);
+  }
   // four values of a sum at a time, the threads' next to each other
   const int nt = blockDim.x;
   float4* held = (float4*)fold + threadIdx.x;
@@ -327,7 +364,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
 #pragma unroll
   for (int k = 0; k < V; ++k) ones[k] = 1.f;
   const int64_t step = (int64_t)gridDim.x * RPB;
-  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  int64_t row = (int64_t)xcd_remap(blockIdx.x, gridDim.x) * RPB + threadIdx.x / TPR;
   uint4 rx[NIT], ry[NIT], rz[NIT], rd[NIT], rm[NIT];
   float4 rs;
 #pragma unroll
@@ -340,6 +377,26 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
     if (a.dr) load_row<T>(C, (const T*)a.dr + at * a.lddr, rd);
     if (a.dh) load_row<T>(C, (const T*)a.dh + at * a.lddh, rm);
   };
+#pragma unroll
+  for (int i = 0; i < NIT; ++i) {
+    const int c = min(C.at(i), max(a.D - V, 0));
+    if constexpr (IN) {
+      float s[V], g[V];
+      vec_chunk(a.scale, wb, c, a.D, 1.f, s);
+      vec_chunk(a.post_w, wb, c, a.D, 1.f, P[i]);
+      vec_chunk(BIAS ? a.post_b : nullptr, wb, c, a.D, 0.f, Q[i]);
+      if (a.gate_mode == GNNEA_GATE_ROW) vec_chunk(a.gate, wb, c, a.D, 0.f, g);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        s[k] *= a.alpha;
+        if (a.gate_mode == GNNEA_GATE_ROW) s[k] *= gate_of(g[k]).g;
+        P[i][k] *= s[k];
+        Q[i][k] *= s[k];
+      }
+    }
+    vec_chunk(a.pre_w, wb, c, a.D, 1.f, W[i]);
+  }
+  // (after the vectors: before them the loop came out 20 % slower at 8191 rows of 4097 bf16)
   if (kAhead && row < a.n) load(row);
   for (; row < a.n; row += step) {
     if (!kAhead) load(row);
@@ -429,21 +486,23 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
     }
   }
   if (!a.part) return;
-  // the workgroup's column sums: over its rows in row order, one of the four after another
+  // the workgroup's column sums
+  if constexpr (kLds) {
+    // lanes over the 64 values of 16 columns, each from the place of the thread that holds it
+    __syncthreads();
+    for (int e = threadIdx.x; e < (C.D + 15) / 16 * 64; e += nt) {
+      const int c = (e >> 6) * 16 + (e & 15), q = (e >> 4) & 3;
+      if (c >= C.D || !(a.sums & (1 << q))) continue;
+      const int chunk = c / V, k = c - min(chunk * V, C.D - V);
+      a.part[part_at(c, blockIdx.x, gridDim.x, q)] =
+          fold[(((q * NIT + chunk / nt) * (V / 4) + k / 4) * nt + chunk % nt) * 4 + k % 4];
+    }
+  } else {
+    // over its rows in row order, one sum after another
+    constexpr int kRow = TPR * NIT * V;  // (of LDS, for each of the workgroup's rows)
 #pragma unroll
-  for (int q = 0; q < kNormSums; ++q) {
-    if (!(a.sums & (1 << q))) continue;
-    float* out = a.part + ((int64_t)blockIdx.x * kNormSums + q) * C.D;
-    if constexpr (RPB == 1) {
-#pragma unroll
-      for (int i = 0; i < NIT; ++i)
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (C.has(i) && C.own(i, k))
-            out[C.at(i) + k] =
-                fold[(((q * NIT + i) * (V / 4) + k / 4) * nt + threadIdx.x) * 4 + k % 4];
-    } else {
-      constexpr int kRow = TPR * NIT * V;  // (of LDS, for each of the workgroup's rows)
+    for (int q = 0; q < kNormSums; ++q) {
+      if (!(a.sums & (1 << q))) continue;
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < NIT; ++i)
@@ -455,53 +514,50 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
       for (int c = threadIdx.x; c < C.D; c += 256) {
         float s = fold[c];
         for (int w = 1; w < RPB; ++w) s += fold[w * kRow + c];
-        out[c] = s;
+        a.part[part_at(c, blockIdx.x, gridDim.x, q)] = s;
       }
     }
   }
 }
 
 // The workgroups' column sums in a fixed order (fp64), and the six vector gradients from them.  16
-// columns per workgroup; 64 groups of 16 lanes take every 64th partial row.
+// columns per workgroup: a wave reads the four sums of one workgroup, 16 waves every 16th.
 __global__ __launch_bounds__(1024) void k_norm_fold(const gnnea_norm a, int blocks) {
-  __shared__ double sh[kNormSums][64][17];
-  const int lc = threadIdx.x & 15, w = threadIdx.x >> 4, c = blockIdx.x * 16 + lc;
+  __shared__ double sh[16][64];
+  const int lc = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3, w = wave_id();
+  const int c = blockIdx.x * 16 + lc;
   const bool in = c < a.D, wb = a.w_dtype == GNNEA_BF16;
-  double s[kNormSums] = {0.0, 0.0, 0.0, 0.0};
   float scale = 0.f, gate = 0.f, pw = 0.f, pb = 0.f;
-  if (in) {
+  if (in && threadIdx.x < 16) {
     scale = a.alpha * vec_at(a.scale, wb, c, 1.f);
     gate = a.gate_mode == GNNEA_GATE_ROW ? vec_at(a.gate, wb, c, 0.f) : 0.f;
     pw = vec_at(a.post_w, wb, c, 1.f);
     pb = vec_at(a.post_b, wb, c, 0.f);
-    for (int b = w; b < blocks; b += 64 * 4) {
-      float v[4][kNormSums];
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int q = 0; q < kNormSums; ++q)
-          v[u][q] = (a.sums & (1 << q)) && b + 64 * u < blocks
-                        ? a.part[((int64_t)(b + 64 * u) * kNormSums + q) * a.D + c] : 0.f;
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int q = 0; q < kNormSums; ++q) s[q] += (double)v[u][q];
-    }
   }
+  double s = 0.0;
+  if (in && (a.sums & (1 << q))) {
+    const float* p = a.part + part_at(c, 0, blocks, q);
+    int b = w;
+    for (; b + 112 < blocks; b += 128) {
+      float v[8];
 #pragma unroll
-  for (int q = 0; q < kNormSums; ++q) sh[q][w][lc] = s[q];
+      for (int u = 0; u < 8; ++u) v[u] = p[(int64_t)(b + 16 * u) * 64];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += (double)v[u];
+    }
+    for (; b < blocks; b += 16) s += (double)p[(int64_t)b * 64];
+  }
+  sh[w][lane_id()] = s;
   __syncthreads();
-  if (threadIdx.x < 64) {  // 16 columns x the four sums
-    const int q = threadIdx.x >> 4;
-    double t = sh[q][0][lc];
-    for (int k = 1; k < 64; ++k) t += sh[q][k][lc];
-    sh[q][0][lc] = t;
+  if (w == 0) {
+    for (int k = 1; k < 16; ++k) s += sh[k][lane_id()];
+    sh[0][lane_id()] = s;
   }
   __syncthreads();
   if (threadIdx.x >= 16 || !in) return;
   float got[kNormSums];
 #pragma unroll
-  for (int q = 0; q < kNormSums; ++q) got[q] = (float)sh[q][0][lc];
+  for (int k = 0; k < kNormSums; ++k) got[k] = (float)sh[0][16 * k + lc];
   auto put = [&](void* p, float v) {
     if (!p) return;
     if (wb) ((bf16_t*)p)[c] = f32_to_bf16(v);
@@ -538,12 +594,23 @@ static NormPlan norm_plan(int64_t n, int D, int V, bool bwd) {
   const int rpb = p.tpr < 256 ? 256 / p.tpr : 1, waves = p.threads / 64;
   // (backward: two rows at least, so that the column sums stay few)
   const int64_t want = bwd ? (n + 2 * rpb - 1) / (2 * rpb) : (n + rpb - 1) / rpb;
-  // rows per workgroup go up with n: the workgroups fill the chip once, and each reads its next
-  // row while it computes one
-  const int fit = bwd ? (waves <= 4 ? 2 : 1) : waves <= 5 ? 4 : waves <= 10 ? 2 : 1;
-  const int64_t cap = 256 * fit;
+  // As many workgroups as fit the chip at once, each with many rows, the next one always on its
+  // way.  Where rows are many, more workgroups of 16 (backward: 128) rows a wave even the chip out:
+  // 1M rows of 300 fp32, forward 1307 us with 1024 workgroups, 1264 with 4096, 1220 with 16384;
+  // backward 2079 with 512, 2026 with 2048 (its column sums' fold goes from 6 to 14).
+  int64_t cap = 256 * (waves <= 4 ? (bwd ? 2 : 4) : bwd ? 1 : waves <= 5 ? 4 : waves <= 10 ? 2 : 1);
+  if (waves <= 4) {
+    int64_t more = n / ((bwd ? 128 : 16) * rpb);
+    const int64_t most = bwd ? 2048 : 16384;
+    more = more < most ? more : most;
+    cap = cap > more ? cap : more;
+  }
   p.blocks = (int)(want < cap ? want : cap);
   return p;
+}
+
+static int64_t norm_ws(const NormPlan& p, int D) {
+  return (int64_t)div_up(D, 16) * 16 * p.blocks * kNormSums * 4;
 }
 
 static int norm_check(const gnnea_norm* a, bool bwd) {
@@ -647,7 +714,7 @@ extern "C" int gnnea_norm_fwd(const gnnea_norm* arg, void* stream) {
 extern "C" int64_t gnnea_norm_bwd_ws_bytes(int64_t n, int32_t D, int dtype) {
   if (n < 0 || D < 1 || D > kNormMaxD || (dtype != GNNEA_F32 && dtype != GNNEA_BF16))
     return GNNEA_EINVAL;
-  return (int64_t)norm_plan(n, D, dtype == GNNEA_F32 ? 4 : 8, true).blocks * kNormSums * D * 4;
+  return norm_ws(norm_plan(n, D, dtype == GNNEA_F32 ? 4 : 8, true), D);
 }
 
 extern "C" int gnnea_norm_bwd(const gnnea_norm* arg, void* ws, int64_t ws_bytes, void* stream) {
@@ -658,7 +725,7 @@ extern "C" int gnnea_norm_bwd(const gnnea_norm* arg, void* ws, int64_t ws_bytes,
   const NormPlan p = norm_plan(a.n, a.D, a.dtype == GNNEA_F32 ? 4 : 8, true);
   a.part = nullptr;
   if (a.sums) {
-    if (ws_bytes < (int64_t)p.blocks * kNormSums * a.D * 4) return GNNEA_EWORKSPACE;
+    if (ws_bytes < norm_ws(p, a.D)) return GNNEA_EWORKSPACE;
     if (p.blocks && (!ws || ((uintptr_t)ws & 15))) return ws ? GNNEA_EALIGN : GNNEA_EINVAL;
     a.part = (float*)ws;
   }
