@@ -196,15 +196,17 @@ template <int NCH> struct Steps { static constexpr int U = NCH <= 2 ? 2 : 1; };
 // The next 64 columns of the unit's entries, one per lane, read while the current ones are used.
 // Lanes past the end repeat the last entry: what is read for them is the row's own, and weighs 0.
 struct ColBatch {
-  int now, next, left;
-  __device__ __forceinline__ ColBatch(const int32_t* col, int beg, int end) {
-    next = now = left = 0;
-    if (beg < end) next = col[min(beg + lane_id(), end - 1)];
+  const int32_t* col;  // the unit's first
+  int total, now, next, left;
+  __device__ __forceinline__ ColBatch(const gnnea_attn& a, const AttnUnit& u)
+      : col(a.col + u.beg), total(u.end - u.beg), now(0), next(0), left(0) {
+    if (total > 0) next = col[min(lane_id(), total - 1)];
   }
-  __device__ __forceinline__ void step(const int32_t* col, int at, int end) {
+  __device__ __forceinline__ void step(uint32_t done) {
     now = next;
-    left = min(end - at, 64);
-    if (at + 64 < end) next = col[min(at + 64 + lane_id(), end - 1)];
+    const int rest = total - (int)done;
+    left = min(rest, 64);
+    if (rest > 64) next = col[(int64_t)done + min(64 + lane_id(), rest - 1)];
   }
 };
 
@@ -248,14 +250,14 @@ __global__ __launch_bounds__(256) void k_attn_fwd(const gnnea_attn a, int hpw,
   uint4 q[NCH];
   float o[NCH][V], m, sum;
   for (bool care = false;; care = true) {
-    ColBatch cb(a.col, u.beg, u.end);
+    ColBatch cb(a, u);
     RowOffset off(a.n_cols, a.ldk);
     L.load_own((const T*)a.q + u.row * a.ldq + (int64_t)head * dh, on, q);
     m = -INFINITY;
     sum = 0.f;
     clear(o);
-    for (int at = u.beg; at < u.end; at += 64) {
-      cb.step(a.col, at, u.end);
+    for (uint32_t done = 0; done < (uint32_t)cb.total; done += 64) {
+      cb.step(done);
       off.set(cb.now, a.ldk);
       for (int b = 0; b < cb.left; b += eps * U) {
         uint4 rk[U][NCH], rv[U][NCH];
@@ -287,7 +289,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd(const gnnea_attn a, int hpw,
           top = x[s] > top || x[s] != x[s] ? x[s] : top;
         }
         const float ref = top == -INFINITY ? 0.f : top;  // only -inf so far: all weights are 0
-        if (at + b > u.beg) {                            // (o and sum are 0 before the first)
+        if (done + b > 0) {                              // (o and sum are 0 before the first)
           const float keep = __builtin_amdgcn_exp2f(m - ref);
           sum *= keep;
 #pragma unroll
@@ -350,15 +352,15 @@ __global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, int hpw,
   uint4 q[NCH], d[NCH];
   float A[NCH][V], B[NCH][V], delta;
   for (bool care = false;; care = true) {
-    ColBatch cb(a.col, u.beg, u.end);
+    ColBatch cb(a, u);
     RowOffset off(a.n_cols, a.ldk);
     L.load_own((const T*)a.q + u.row * a.ldq + (int64_t)head * dh, on, q);
     L.load_own((const T*)a.dout + u.row * a.lddo + (int64_t)head * dh, on, d);
     delta = 0.f;
     clear(A);
     clear(B);
-    for (int at = u.beg; at < u.end; at += 64) {
-      cb.step(a.col, at, u.end);
+    for (uint32_t done = 0; done < (uint32_t)cb.total; done += 64) {
+      cb.step(done);
       off.set(cb.now, a.ldk);
       for (int b = 0; b < cb.left; b += eps * U) {
         uint4 rk[U][NCH], rv[U][NCH];
@@ -444,14 +446,14 @@ __global__ __launch_bounds__(256) void k_attn_cols(const gnnea_attn a, int hpw,
   uint4 kf[NCH], vf[NCH];
   float dk[NCH][V], dv[NCH][V];
   for (bool care = false;; care = true) {
-    ColBatch cb(a.col, u.beg, u.end);
+    ColBatch cb(a, u);
     RowOffset offq(a.n_cols, a.ldq), offd(a.n_cols, a.lddo);
     L.load_own((const T*)a.k + u.row * a.ldk + (int64_t)kvh * dh, on, kf);
     L.load_own((const T*)a.v + u.row * a.ldv + (int64_t)kvh * dh, on, vf);
     clear(dk);
     clear(dv);
-    for (int at = u.beg; at < u.end; at += 64) {
-      cb.step(a.col, at, u.end);
+    for (uint32_t done = 0; done < (uint32_t)cb.total; done += 64) {
+      cb.step(done);
       offq.set(cb.now, a.ldq);
       offd.set(cb.now, a.lddo);
       const int pairs = cb.left * share;  // share <= heads <= 65535: fits

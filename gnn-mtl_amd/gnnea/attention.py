@@ -23,20 +23,21 @@ class _Pieces:
     """The pieces of a CSR's long rows (they depend on rowptr alone; built once per matrix)."""
 
     def __init__(self, csr):
-        deg = csr.degrees().long()
-        rows = torch.nonzero(deg > LONG_ROW).flatten()  # one setup sync
+        deg, limit = csr.degrees().long(), LONG_ROW
+        rows = torch.nonzero(deg > limit).flatten()  # one setup sync
+        self.limit = limit
         self.n_long = int(rows.numel())
         self.n_items = 0
         self.rows = self.ptr = self.items = None
         if self.n_long:
-            count = (deg[rows] + LONG_ROW - 1) // LONG_ROW
+            count = (deg[rows] + limit - 1) // limit
             end = torch.cumsum(count, 0)
             self.n_items = int(end[-1])
             which = torch.repeat_interleave(torch.arange(self.n_long, device=rows.device), count)
             slot = torch.arange(self.n_items, device=rows.device)
             row = rows[which]
-            beg = csr.rowptr[row].long() + (slot - (end - count)[which]) * LONG_ROW
-            stop = torch.minimum(beg + LONG_ROW, csr.rowptr[row + 1].long())
+            beg = csr.rowptr[row].long() + (slot - (end - count)[which]) * limit
+            stop = torch.minimum(beg + limit, csr.rowptr[row + 1].long())
             self.items = torch.stack([row, beg, stop, slot], 1).to(torch.int32).contiguous()
             self.rows = rows.to(torch.int32)
             self.ptr = torch.cat([end.new_zeros(1), end]).to(torch.int32)
@@ -57,7 +58,7 @@ def _problem(csr, q, k, v, meta):
     a.n_rows, a.n_cols = csr.n_rows, csr.n_cols
     a.heads, a.kv_heads, a.d_head, a.scale = heads, kv_heads, q.shape[1] // heads, scale
     a.dtype = _lib.GNNEA_BF16 if q.dtype == torch.bfloat16 else _lib.GNNEA_F32
-    a.limit = LONG_ROW
+    a.limit = pieces.limit
     if pieces.n_long:
         a.n_items, a.n_long = pieces.n_items, pieces.n_long
         a.items, a.long_rows, a.long_ptr = (t.data_ptr() for t in (pieces.items, pieces.rows,
@@ -78,17 +79,23 @@ def _run(which, a, device):
         check(fn(a, ptr(ws), ws_bytes, stream_of(device)))
 
 
+def _forward(q, k, v, csr, meta, want_lse):
+    """(out, lse): lse, the rows' log-sum-exp, for a backward pass."""
+    a = _problem(csr, q, k, v, meta)
+    out = torch.empty((q.shape[0], q.shape[1]), dtype=q.dtype, device=q.device)
+    a.o, a.ldo = out.data_ptr(), q.shape[1]
+    lse = None
+    if want_lse:
+        lse = torch.empty((q.shape[0], meta[0]), dtype=torch.float32, device=q.device)
+        a.lse = lse.data_ptr()
+    _run(_lib.GNNEA_ATTN_FWD, a, q.device)
+    return out, lse
+
+
 class DotAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, csr, meta):
-        a = _problem(csr, q, k, v, meta)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        a.o, a.ldo = out.data_ptr(), q.shape[1]
-        lse = None
-        if any(ctx.needs_input_grad):
-            lse = torch.empty((q.shape[0], meta[0]), dtype=torch.float32, device=q.device)
-            a.lse = lse.data_ptr()
-        _run(_lib.GNNEA_ATTN_FWD, a, q.device)
+        out, lse = _forward(q, k, v, csr, meta, any(ctx.needs_input_grad))
         ctx.save_for_backward(q, k, v, lse)
         ctx.csr, ctx.meta = csr, meta
         return out
@@ -136,24 +143,28 @@ def dot_attention(adj, q, k, v, heads, kv_heads=None, scale=None):
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError("gnnea.dot_attention: heads must be a multiple of kv_heads (got %r, %r)"
                          % (heads, kv_heads))
+    dtype, device, d = q.dtype, csr.device, 0
     for name, t, n, h in (("q", q, csr.n_rows, heads), ("k", k, csr.n_cols, kv_heads),
                           ("v", v, csr.n_cols, kv_heads)):
-        if t.dim() != 2 or t.shape[0] != n or t.shape[1] == 0 or t.shape[1] % h or \
-                t.shape[1] // h != q.shape[1] // heads:
+        shape = t.shape
+        if len(shape) != 2 or shape[0] != n or shape[1] == 0 or shape[1] % h or \
+                (d and shape[1] != h * d):
             raise ValueError("gnnea.dot_attention: %s must be [%d, %d * d_head] (got %s)"
-                             % (name, n, h, tuple(t.shape)))
-        if t.dtype not in FEATURE_DTYPES or t.dtype != q.dtype:
+                             % (name, n, h, tuple(shape)))
+        d = shape[1] // h
+        if t.dtype != dtype or dtype not in FEATURE_DTYPES:
             raise TypeError("gnnea.dot_attention: q, k and v must all be fp32 or all bf16 (got %s)"
                             % t.dtype)
-        if t.device != csr.device:
+        if t.device != device:
             raise ValueError("gnnea.dot_attention: %s is on %s, the adjacency on %s"
-                             % (name, t.device, csr.device))
-    d = q.shape[1] // heads
+                             % (name, t.device, device))
     if d > MAX_D_HEAD:
         raise ValueError("gnnea.dot_attention: d_head must be at most %d (got %d)"
                          % (MAX_D_HEAD, d))
-    scale = d ** -0.5 if scale is None else float(scale)
-    k, v = _rows(k), _rows(v)
+    meta = (heads, kv_heads, d ** -0.5 if scale is None else float(scale))
+    q, k, v = _rows(q), _rows(k), _rows(v)
     if _ld(k) != _ld(v):  # the kernels form one row offset for both
         k, v = k.contiguous(), v.contiguous()
-    return DotAttentionFn.apply(_rows(q), k, v, csr, (heads, kv_heads, scale))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return DotAttentionFn.apply(q, k, v, csr, meta)
+    return _forward(q, k, v, csr, meta, False)[0]

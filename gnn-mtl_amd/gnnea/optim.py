@@ -65,11 +65,17 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, group):
         self._base.append(sum(len(g["params"]) for g in self.param_groups))
         super().add_param_group(group)
+        if len(set(map(id, self.param_groups[-1]["params"]))) != len(self.param_groups[-1]["params"]):
+            raise ValueError("gnnea.AdamW: a parameter is in its group twice")
         for p in self.param_groups[-1]["params"]:
             if p.dtype not in FEATURE_DTYPES:
                 raise TypeError("gnnea.AdamW: fp32 or bf16 parameters required (got %s)" % p.dtype)
             if p.is_sparse or not _dense(p):
                 raise ValueError("gnnea.AdamW: parameters must be dense and without gaps")
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), state_bits=self.state_bits, max_norm=self.max_norm,
+                    seed=self.seed, grad_norm=None, _base=self._base)
 
     def _init_state(self, p, step):
         if torch.cuda.is_current_stream_capturing():
@@ -169,6 +175,9 @@ class AdamW(torch.optim.Optimizer):
             for group, step, arrays in groups:
                 lr, (b1, b2) = group["lr"], group["betas"]
                 on_device = isinstance(lr, torch.Tensor)
+                if on_device and lr.device != device:
+                    raise ValueError("gnnea.AdamW: lr is on %s, the parameters on %s"
+                                     % (lr.device, device))
                 ctl = torch.empty(_lib.GNNEA_ADAMW_CTL_BYTES // 4, dtype=torch.float32,
                                   device=device)
                 check(L.gnnea_adamw_begin(ptr(parts), n_parts, self.max_norm or 0.0, b1, b2,
@@ -208,6 +217,7 @@ class AdamW(torch.optim.Optimizer):
                                                      stream_of(device)))
         return out
 
+    @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Takes the state as it is (codes stay uint8, moments of bf16 parameters stay fp32)."""
         saved = state_dict["param_groups"]
@@ -220,30 +230,36 @@ class AdamW(torch.optim.Optimizer):
         new = {}
         for old, group in zip(saved, self.param_groups):
             ps = dict(zip(old["params"], group["params"]))
-            step = None
+            # (what is there is written into: a captured step keeps its addresses)
+            step = next((self.state[p]["step"] for p in group["params"] if p in self.state), None)
             for key, p in ps.items():
                 got = state_dict["state"].get(key)
                 if not got:
                     continue
-                if step is None:
-                    step = torch.as_tensor(got["step"]).reshape(1).to(torch.int64, copy=True).to(
-                        p.device)
+                t = torch.as_tensor(got["step"]).reshape(1).to(torch.int64)
+                step = t.to(p.device, copy=True) if step is None else step.copy_(t)
                 n = p.numel()
                 shapes = dict(exp_avg=p.shape if self.state_bits == 32 else (n,),
                               exp_avg_sq=p.shape, exp_avg_rms=(n,), scales=(2, -(-n // BLOCK)))
-                s = dict(step=step)
+                have, s = self.state.get(p), dict(step=step)
                 for name in names:
                     t = got.get(name)
                     if t is None or t.dtype != dtype or tuple(t.shape) != tuple(shapes[name]):
                         raise ValueError("gnnea.AdamW: %s of parameter %s must be %s %s for "
                                          "state_bits=%d" % (name, key, tuple(shapes[name]), dtype,
                                                             self.state_bits))
-                    like = p if t.dim() == p.dim() and t.shape == p.shape and \
-                        self.state_bits == 32 else None
-                    s[name] = torch.empty_like(like, dtype=dtype) if like is not None else \
-                        torch.empty(t.shape, dtype=dtype, device=p.device)
+                    if have is not None:
+                        s[name] = have[name]
+                    elif self.state_bits == 32:
+                        s[name] = torch.empty_like(p, dtype=dtype)
+                    else:
+                        s[name] = torch.empty(t.shape, dtype=dtype, device=p.device)
                     s[name].copy_(t)
                 new[p] = s
-            group.update({k: v for k, v in old.items() if k != "params"})
+            for k, v in old.items():
+                if k == "lr" and isinstance(group["lr"], torch.Tensor):
+                    group["lr"].copy_(torch.as_tensor(v).reshape(group["lr"].shape))
+                elif k != "params":
+                    group[k] = float(v) if isinstance(v, torch.Tensor) else v
         self.state.clear()
         self.state.update(new)

@@ -279,3 +279,35 @@ def test_refusals(device):
         qq = q.clone().requires_grad_()
         gq, = torch.autograd.grad(dot_attention(adj, qq, k, v, 2).sum(), qq, create_graph=True)
         gq.sum().backward()
+
+
+def test_offsets_past_32_bits(device):
+    """Keys and values whose elements lie past 2^32 in their buffer (17M rows, 256 apart): the same
+    bits as from a small buffer."""
+    from gnnea.attention import dot_attention
+    from gnnea.graph import DeviceCSR
+    n, ld = 17_000_000, 256
+    wide = torch.zeros(n, ld, dtype=torch.bfloat16, device=device)
+    g = torch.Generator().manual_seed(4)
+    cols = torch.tensor([0, 5, n - 300, n - 2, n - 1])
+    kv = torch.randn(5, 32, generator=g).bfloat16().to(device)
+    wide[cols.to(device), :32] = kv
+    row = torch.tensor([0, 0, 1, 1, 1, 2])
+    pick = torch.tensor([0, 3, 1, 2, 4, 4])
+    q = torch.randn(3, 16, generator=g).bfloat16().to(device)
+    do = torch.randn(3, 16, generator=g).bfloat16().to(device)
+    far = DeviceCSR.from_coo(row.to(device), cols[pick].to(device), None, 3, n)
+    near = DeviceCSR.from_coo(row.to(device), pick.to(device), None, 3, 5)
+    out = dot_attention(far, q, wide[:, :16], wide[:, 16:32], 2)
+    assert torch.equal(out, dot_attention(near, q, kv[:, :16], kv[:, 16:], 2))
+    # queries past 2^32: the transposed matrix gathers them
+    back = DeviceCSR.from_coo(cols[pick].to(device), row.to(device), None, n, 3)
+    small = DeviceCSR.from_coo(pick.to(device), row.to(device), None, 5, 3)
+    Q = wide[:, :16].detach().requires_grad_()
+    D = torch.zeros(n, 16, dtype=torch.bfloat16, device=device)
+    D[cols.to(device)] = kv[:, 16:]
+    k = q.clone().requires_grad_()
+    got = torch.autograd.grad(dot_attention(back, Q, k, do, 2), (Q, k), D)
+    Qs, ks = kv[:, :16].detach().clone().requires_grad_(), q.clone().requires_grad_()
+    want = torch.autograd.grad(dot_attention(small, Qs, ks, do, 2), (Qs, ks), kv[:, 16:].contiguous())
+    assert torch.equal(got[1], want[1]) and torch.equal(got[0][cols.to(device)], want[0])

@@ -283,3 +283,27 @@ def test_refusals(device):
         norm(torch.ones(2, 8193, device=device))
     with pytest.raises(ValueError):
         norm(torch.ones(2, 3, 8, device=device))
+
+
+def test_offsets_past_32_bits(device):
+    """8M rows of 300 (2.4e9 elements): the last rows as from a small call, column sums of a
+    constant exact (every sum of the call is a whole number below 2^24)."""
+    from gnnea.norm import residual_norm
+    n, D = 8_000_000, 300
+    x = torch.zeros(n, D, dtype=torch.bfloat16, device=device)
+    y = torch.ones(n, D, dtype=torch.bfloat16, device=device)
+    g = torch.Generator().manual_seed(0)
+    x[-70:] = torch.randn(70, D, generator=g).bfloat16().to(device)
+    y[-70:] = torch.randn(70, D, generator=g).bfloat16().to(device)
+    w = torch.ones(D, device=device)
+    r, h = residual_norm(x, y, scale=0.5, post_weight=w, pre_weight=w)
+    r2, h2 = residual_norm(x[-70:], y[-70:], scale=0.5, post_weight=w, pre_weight=w)
+    assert torch.equal(r[-70:], r2) and torch.equal(h[-70:], h2)
+    del r, h
+    b = torch.zeros(D, device=device, requires_grad=True)
+    y.requires_grad_()
+    r, _ = residual_norm(x, y, post_weight=w, post_bias=b, pre=False, kind="layer")
+    dr = torch.ones(1, 1, dtype=torch.bfloat16, device=device).expand(n, D).contiguous()
+    db, dy = torch.autograd.grad(r, (b, y), dr)
+    assert bool((db == n).all())
+    assert bool((dy[-70:].float().abs() <= 2.0 ** -8).all())  # a constant's gradient through N is 0

@@ -332,3 +332,47 @@ def test_refusals(device):
     with pytest.raises(RuntimeError):
         with torch.cuda.graph(g):
             first.step()
+
+
+def test_offsets_past_32_bits(device):
+    """A bf16 tensor of 2^32 + 4097 elements, all alike: all alike after a step, and as a small
+    tensor's."""
+    from gnnea.optim import AdamW
+    got = []
+    for n in (2 ** 32 + 4097, 5):
+        p = torch.nn.Parameter(torch.full((n,), 1.5, dtype=torch.bfloat16, device=device))
+        p.grad = torch.full_like(p, 0.25)
+        opt = AdamW([p], lr=0.1, max_norm=None)
+        opt.step()
+        m, v = opt.moments()[0]
+        for t in (p.detach(), m, v):
+            lo, hi = torch.aminmax(t)
+            assert lo == hi
+        got.append((p.detach()[-1].item(), m[-1].item(), v[-1].item()))
+        del p, opt, m, v, t
+        torch.cuda.empty_cache()
+    assert got[0] == got[1]
+
+
+def test_copies_duplicates_and_rates(device):
+    """A deep copy goes on by itself; the same parameter twice, and a rate on the host, are refused;
+    loading writes into the state that is there."""
+    from gnnea.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(300, device=device))
+    with pytest.raises(ValueError):
+        AdamW([p, p])
+    with pytest.raises(ValueError):
+        AdamW([p], lr=torch.ones(1))
+    p.grad = torch.full_like(p, 0.5)
+    opt = AdamW([p], state_bits=8, max_norm=1.0)
+    opt.step()
+    twin = copy.deepcopy(opt)
+    q = twin.param_groups[0]["params"][0]
+    q.grad = p.grad.clone()
+    opt.step()
+    twin.step()
+    assert torch.equal(p, q)
+    where = opt.state[p]["exp_avg"].data_ptr(), opt.state[p]["step"].data_ptr()
+    opt.load_state_dict(copy.deepcopy(twin.state_dict()))
+    assert where == (opt.state[p]["exp_avg"].data_ptr(), opt.state[p]["step"].data_ptr())
+    assert int(opt.state[p]["step"]) == 2
