@@ -244,7 +244,7 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamList L, const AdamHyper
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      p[u][k] = p[u][k] * decay - lr1 * m[u][k] / (root[k] * s.bc2 + h.eps);
+      p[u][k] = p[u][k] * decay - lr1 * m[u][k] * __builtin_amdgcn_rcpf(root[k] * s.bc2 + h.eps);
     store4<T, NT>((T*)t.p + at, left, p[u]);
   }
 }

@@ -27,7 +27,13 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-struct AttnPlan { int lph, nch, hpw, units_y; bool full; };
+// hs: log2 of the heads that a wave's groups take at once; share: query heads per key/value head,
+// ss: its log2 where it has one, else -1
+struct AttnPlan { int lph, nch, hs, share, ss, units_y; bool full; };
+struct AttnShape { int hs, share, ss; };
+__device__ __forceinline__ int by_share(const AttnShape& p, int x) {
+  return p.ss >= 0 ? x >> p.ss : (int)((uint32_t)x / (uint32_t)p.share);
+}
 
 // The 16-B chunks of a head that a lane holds: NCH of them, LPH lanes apart.  FULL: d_head is
 // LPH NCH V.  Otherwise a head's last chunk is moved back so that it ends with the head, and holds
@@ -234,16 +240,16 @@ struct RowOffset {
 // whose sums came out not finite, with 0 in every place that is not an entry's own (0 times an
 // infinity read for nothing is not 0).
 template <typename T, int LPH, int NCH, bool FULL>
-__global__ __launch_bounds__(256) void k_attn_fwd(const gnnea_attn a, int hpw,
+__global__ __launch_bounds__(256) void k_attn_fwd(const gnnea_attn a, const AttnShape S,
                                                   float* __restrict__ ws) {
   constexpr int V = RowChunk<T>::V, G = 64 / LPH, U = Steps<NCH>::U;
   AttnUnit u;
   if (!attn_unit(a, u)) return;
   const int lane = lane_id(), grp = lane / LPH, dh = a.d_head;
   const Lane<T, LPH, NCH, FULL> L{dh, lane % LPH};
-  const int head = blockIdx.y * hpw + grp % hpw, slot = grp / hpw, eps = G / hpw;
+  const int head = (blockIdx.y << S.hs) + (grp & ((1 << S.hs) - 1)), slot = grp >> S.hs, eps = G >> S.hs;
   const bool on = head < a.heads;
-  const int64_t kvo = (int64_t)(on ? head / (a.heads / a.kv_heads) : 0) * dh;
+  const int64_t kvo = (int64_t)(on ? by_share(S, head) : 0) * dh;
   const T* K = (const T*)a.k + kvo;
   const T* Vp = (const T*)a.v + kvo;
   const float factor = a.scale * kLog2e;
@@ -281,23 +287,26 @@ __global__ __launch_bounds__(256) void k_attn_fwd(const gnnea_attn a, int hpw,
               rv[s][c] = L.mask(rv[s][c], c, ok[s]);
             }
         }
-        float x[U], top = m;
+        float x[U], top = -INFINITY;
 #pragma unroll
         for (int s = 0; s < U; ++s) {
           const float d = head_dot<V, LPH>(q, rk[s]) * factor;
           x[s] = ok[s] ? d : -INFINITY;
           top = x[s] > top || x[s] != x[s] ? x[s] : top;
         }
-        const float ref = top == -INFINITY ? 0.f : top;  // only -inf so far: all weights are 0
-        if (done + b > 0) {                              // (o and sum are 0 before the first)
-          const float keep = __builtin_amdgcn_exp2f(m - ref);
+        // The reference moves when a score is over it by more than 2^8 in weight: sums of weights
+        // up to that stay exact enough in fp32, and most entries leave o and sum as they are.
+        if (__any(!(top <= m + 8.f))) {
+          const float to = !(top <= m + 8.f) ? top : m;
+          const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
+          m = to;
           sum *= keep;
 #pragma unroll
           for (int c = 0; c < NCH; ++c)
 #pragma unroll
             for (int k = 0; k < V; ++k) o[c][k] *= keep;
         }
-        m = top;
+        const float ref = m == -INFINITY ? 0.f : m;  // only -inf so far: all weights are 0
 #pragma unroll
         for (int s = 0; s < U; ++s) {
           const float p = __builtin_amdgcn_exp2f(x[s] - ref);
@@ -310,7 +319,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd(const gnnea_attn a, int hpw,
     const float z = on ? zero_of(o, sum * 0.f) : 0.f;
     if (care || !__any(z != z)) break;
   }
-  for (int w = LPH * hpw; w < 64; w <<= 1) {  // the groups of one head
+  for (int w = LPH << S.hs; w < 64; w <<= 1) {  // the groups of one head
     const float mo = lane_xor(m, w), so = lane_xor(sum, w);
     const float top = mo > m || mo != mo ? mo : m;
     const float ref = top == -INFINITY ? 0.f : top;
@@ -335,16 +344,16 @@ __global__ __launch_bounds__(256) void k_attn_fwd(const gnnea_attn a, int hpw,
 }
 
 template <typename T, int LPH, int NCH, bool FULL>
-__global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, int hpw,
+__global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, const AttnShape S,
                                                    float* __restrict__ ws) {
   constexpr int V = RowChunk<T>::V, G = 64 / LPH, U = Steps<NCH>::U;
   AttnUnit u;
   if (!attn_unit(a, u)) return;
   const int lane = lane_id(), grp = lane / LPH, dh = a.d_head;
   const Lane<T, LPH, NCH, FULL> L{dh, lane % LPH};
-  const int head = blockIdx.y * hpw + grp % hpw, slot = grp / hpw, eps = G / hpw;
+  const int head = (blockIdx.y << S.hs) + (grp & ((1 << S.hs) - 1)), slot = grp >> S.hs, eps = G >> S.hs;
   const bool on = head < a.heads;
-  const int64_t kvo = (int64_t)(on ? head / (a.heads / a.kv_heads) : 0) * dh;
+  const int64_t kvo = (int64_t)(on ? by_share(S, head) : 0) * dh;
   const T* K = (const T*)a.k + kvo;
   const T* Vp = (const T*)a.v + kvo;
   const float factor = a.scale * kLog2e;
@@ -402,7 +411,7 @@ __global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, int hpw,
     const float z = on ? zero_of(A, zero_of(B, delta * 0.f)) : 0.f;
     if (care || !__any(z != z)) break;
   }
-  for (int w = LPH * hpw; w < 64; w <<= 1) {
+  for (int w = LPH << S.hs; w < 64; w <<= 1) {
     delta += lane_xor(delta, w);
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
@@ -432,16 +441,15 @@ __global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, int hpw,
 // Columns: a row of the transposed matrix per wave; groups take key/value heads, then (entry,
 // query head of the group) pairs.
 template <typename T, int LPH, int NCH, bool FULL>
-__global__ __launch_bounds__(256) void k_attn_cols(const gnnea_attn a, int hpw,
+__global__ __launch_bounds__(256) void k_attn_cols(const gnnea_attn a, const AttnShape S,
                                                    float* __restrict__ ws) {
   constexpr int V = RowChunk<T>::V, G = 64 / LPH, U = Steps<NCH>::U;
   AttnUnit u;
   if (!attn_unit(a, u)) return;
   const int lane = lane_id(), grp = lane / LPH, dh = a.d_head;
   const Lane<T, LPH, NCH, FULL> L{dh, lane % LPH};
-  const int kvh = blockIdx.y * hpw + grp % hpw, slot = grp / hpw, pps = G / hpw;
+  const int kvh = (blockIdx.y << S.hs) + (grp & ((1 << S.hs) - 1)), slot = grp >> S.hs, pps = G >> S.hs;
   const bool on = kvh < a.kv_heads;
-  const int share = a.heads / a.kv_heads;
   const float factor = a.scale * kLog2e;
   uint4 kf[NCH], vf[NCH];
   float dk[NCH][V], dv[NCH][V];
@@ -456,7 +464,7 @@ __global__ __launch_bounds__(256) void k_attn_cols(const gnnea_attn a, int hpw,
       cb.step(done);
       offq.set(cb.now, a.ldq);
       offd.set(cb.now, a.lddo);
-      const int pairs = cb.left * share;  // share <= heads <= 65535: fits
+      const int pairs = cb.left * S.share;  // share <= heads <= 65535: fits
       for (int b = 0; b < pairs; b += pps * U) {
         uint4 rq[U][NCH], rd[U][NCH];
         float2 st[U];
@@ -465,8 +473,7 @@ __global__ __launch_bounds__(256) void k_attn_cols(const gnnea_attn a, int hpw,
         for (int s = 0; s < U; ++s) {
           const int t = b + s * pps + slot, f = min(t, pairs - 1);
           ok[s] = on && t < pairs;
-          const int e = share == 1 ? f : (int)((uint32_t)f / (uint32_t)share);
-          const int h = (on ? kvh : 0) * share + f - e * share;
+          const int e = by_share(S, f), h = (on ? kvh : 0) * S.share + f - e * S.share;
           const uint64_t i = (uint32_t)__shfl(cb.now, e, 64);
           st[s] = *(const float2*)(a.stat + 2 * (i * a.heads + h));
           const T* Q = (const T*)a.q + (offq.of(e) + h * dh);
@@ -502,7 +509,7 @@ __global__ __launch_bounds__(256) void k_attn_cols(const gnnea_attn a, int hpw,
     const float z = on ? zero_of(dk, zero_of(dv, 0.f)) : 0.f;
     if (care || !__any(z != z)) break;
   }
-  for (int w = LPH * hpw; w < 64; w <<= 1) {
+  for (int w = LPH << S.hs; w < 64; w <<= 1) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
@@ -628,7 +635,7 @@ static int attn_check(const gnnea_attn* a, int pass) {
 static AttnPlan attn_plan(const gnnea_attn* a, int pass) {
   static const int kShape[7][2] = {{4, 1}, {8, 1}, {8, 2}, {8, 3}, {16, 2}, {16, 3}, {16, 4}};
   const int V = a->dtype == GNNEA_F32 ? 4 : 8;
-  AttnPlan p = {16, 4, 1, 1, false};
+  AttnPlan p = {16, 4, 0, a->heads / a->kv_heads, -1, 1, false};
   for (const auto& s : kShape)
     if (s[0] * s[1] * V >= a->d_head) {
       p.lph = s[0];
@@ -637,8 +644,10 @@ static AttnPlan attn_plan(const gnnea_attn* a, int pass) {
     }
   p.full = p.lph * p.nch * V == a->d_head;
   const int heads = pass == GNNEA_ATTN_BWD_COLS ? a->kv_heads : a->heads;
-  while (p.hpw < heads && p.hpw < 64 / p.lph) p.hpw *= 2;
-  p.units_y = (heads + p.hpw - 1) / p.hpw;
+  while ((1 << p.hs) < heads && (1 << p.hs) < 64 / p.lph) ++p.hs;
+  p.units_y = (heads + (1 << p.hs) - 1) >> p.hs;
+  for (int k = 0; k < 16; ++k)
+    if (p.share == 1 << k) p.ss = k;
   return p;
 }
 
@@ -646,12 +655,13 @@ template <typename T, int LPH, int NCH, bool FULL>
 static void attn_launch(const gnnea_attn& a, int pass, const AttnPlan& p, float* ws,
                         hipStream_t s) {
   const dim3 grid(div_up(a.n_items, 4) + div_up(a.n_rows, 4), p.units_y);
+  const AttnShape sh = {p.hs, p.share, p.ss};
   if (pass == GNNEA_ATTN_FWD)
-    hipLaunchKernelGGL((k_attn_fwd<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, p.hpw, ws);
+    hipLaunchKernelGGL((k_attn_fwd<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, sh, ws);
   else if (pass == GNNEA_ATTN_BWD_ROWS)
-    hipLaunchKernelGGL((k_attn_rows<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, p.hpw, ws);
+    hipLaunchKernelGGL((k_attn_rows<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, sh, ws);
   else
-    hipLaunchKernelGGL((k_attn_cols<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, p.hpw, ws);
+    hipLaunchKernelGGL((k_attn_cols<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, sh, ws);
 }
 template <typename T, int LPH, int NCH>
 static void attn_launch(const gnnea_attn& a, int pass, const AttnPlan& p, float* ws,

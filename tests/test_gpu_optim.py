@@ -5,7 +5,7 @@ Tolerances (u = 2^-24).  The clipped gradient is off by 2 u (its factor, the pro
     m    b1's term: the constant, the product, the sum, 3 u; g's: 2 + 3 = 5 u
     v    b2's term 3 u; g's: squared 2 * 2 + 1, the constant, the product, the sum, 8 u
     p    m 5, 1 / (1 - b1^t) 1, lr 1, their products 2; the root (8 / 2 + 1), its factor and product 2,
-         eps 1, the division 1, the product with lr 1: 19 u of the update, 3 u of p (decay, product,
+         eps 1, the reciprocal 2 (one last place), its product 1, the product with lr 1: 21 u of the update, 3 u of p (decay, product,
          difference) and eps / 2 of the value for its type
 Codes: every operation of the restatement rounds as the kernel's does
 (fp32 products and sums of the second moment, fp64 for the first), so they are equal.
@@ -106,7 +106,7 @@ def test_32_bits_against_fp64(device, dtype, max_norm):
             want = before[i] * (1 - 3e-4) - up
             ma = 3e-3 * (((B1 * old[i][0]).abs() + 0.1 * gi.abs()) / (1 - B1 ** t)) / (
                 (v64[i] / (1 - B2 ** t)).sqrt() + 1e-8)
-            tol = 3 * U * before[i].abs() + 19 * U * ma + torch.finfo(dtype).eps / 2 * want.abs()
+            tol = 3 * U * before[i].abs() + 21 * U * ma + torch.finfo(dtype).eps / 2 * want.abs()
             assert bool(((p.detach().double().cpu() - want).abs() <= tol + 1e-38).all()), (t, i)
             # what the next step starts from
             m64[i], v64[i] = m.double().cpu(), v.double().cpu()
@@ -148,7 +148,7 @@ def test_8_bit_codes(device, dtype):
                 u.astype(np.float64) / np.sqrt(1 - B2 ** t) + 1e-8)
             b = before[i].numpy().reshape(-1)
             want = b * (1 - 3e-4) - up
-            tol = 3 * U * np.abs(b) + 19 * U * np.abs(up) + torch.finfo(dtype).eps / 2 * np.abs(want)
+            tol = 3 * U * np.abs(b) + 21 * U * np.abs(up) + torch.finfo(dtype).eps / 2 * np.abs(want)
             got = p.detach().double().cpu().numpy().reshape(-1)
             assert (np.abs(got - want) <= tol + 1e-38).all(), (t, i)
             have[i] = (mq, uq, sc)

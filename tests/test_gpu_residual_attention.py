@@ -99,10 +99,10 @@ def test_ea_iteration_eager_and_replayed(device, model, optim, options):
 
 def test_training_steps_against_torch_adam(device):
     """Five steps of a residual attention encoder under AdamW without decay and under torch's Adam:
-    the same weights.  An update is at most lr (1 + 19 u) however small the gradient, and Adam's
+    the same weights.  An update is at most lr (1 + 21 u) however small the gradient, and Adam's
     first steps magnify a gradient's relative error where the gradient itself is near 0; so the
-    gradients are given, not computed, and the weights differ by 19 u lr a step at most, plus
-    rounding of the weight: 5 (19 u lr + 2 u |w|)."""
+    gradients are given, not computed, and the weights differ by 21 u lr a step at most, plus
+    rounding of the weight: 5 (21 u lr + 2 u |w|)."""
     from gnnea.optim import AdamW
     from models.encoders import GAT
     torch.manual_seed(5)
@@ -120,7 +120,7 @@ def test_training_steps_against_torch_adam(device):
     u = 2.0 ** -24
     for p, q in zip(ps, qs):
         # both sides err
-        tol = 2 * 5 * (19 * u * 1e-2 + 2 * u * q.detach().abs())
+        tol = 2 * 5 * (21 * u * 1e-2 + 2 * u * q.detach().abs())
         assert bool(((p - q).detach().abs() <= tol).all())
 
 
