@@ -20,8 +20,18 @@
 // dr, dh in, dx, dy[, dz] out.  The kernels are bound by HBM.  The backward recomputes r in fp32
 // from x and y instead of reading the stored r: the same bytes, and bf16 storage loses nothing.
 //
-// A row is held by TPR threads (16 lanes, a wave, or a workgroup of 256 or 512), NIT chunks of
-// 16 B per thread; rows of odd widths use the same 16-B accesses at the element's alignment.
+// A row is held by TPR threads (16 lanes, a wave, or as many waves as leave 8 values to a thread),
+// NIT chunks of 16 B per thread; rows of odd widths use the same 16-B accesses at the element's
+// alignment.  A thread keeps its columns from row to row, so the vectors are read once per thread
+// and the column sums stay with it (registers; LDS where a row takes a workgroup, whose registers
+// are full), and the next row is read while one is computed.  Per-row reads of the vectors and
+// element-wise tails had cost 1.9x: 1M rows of 300 fp32, training pass 5.08 ms, now 3.27.
+//
+// Measured: 1M x 300 fp32 with a full gate, forward 1.20 ms (6.0 GB, 5.0 TB/s), backward 2.03
+// (9.6 GB, 4.7 TB/s); 8191 x 4097 bf16 LayerNorm, forward 93 us, backward 123 (2.9, 3.3 TB/s: a
+// row's exchange between waves waits with nothing else to run); 30000 x 300 bf16 forward 22 us
+// (4.1 TB/s); 2000 x 300 7 + 10 + 5 us of launches.
+//
 // Statistics, sums and gradients are fp32; the column sums go per thread over its rows, then over
 // the workgroup's rows, then over workgroups (fp64) in a fixed order: results do not change from
 // run to run.
