@@ -96,6 +96,11 @@ template <int TPR, int NIT, int V> struct Cols {
     const int c = want(i);
     return D >= V && c > D - V ? D - V : c;
   }
+  // whether every value of the wave's chunks is its thread's own (uniform): then no sum needs masks
+  __device__ __forceinline__ bool whole() const {
+    return TPR > 16 && __builtin_amdgcn_readfirstlane(
+        (int)(want(NIT - 1) - lane_id() * V + 64 * V <= D));
+  }
   // whether value k of chunk i is the thread's own: all are, but in a row's last chunk
   __device__ __forceinline__ bool own(int i, int k) const {
     if (i < NIT - 1) return true;
@@ -132,17 +137,24 @@ __device__ __forceinline__ void store_row(const Cols<TPR, NIT, V>& C, T* p, int 
   else store_chunk<T, V>(p, C.D, f);
 }
 
+// the sum over each row of 16 lanes, in all of them
+__device__ __forceinline__ float sum16(float v) {
+  v += mov_dpp_f32<0xB1>(v);
+  v += mov_dpp_f32<0x4E>(v);
+  v += mov_dpp_f32<0x141>(v);
+  v += mov_dpp_f32<0x140>(v);
+  return v;
+}
+
 // Sums of NS values over the TPR threads of a row; every thread gets them, from the same order of
 // additions.  16 lanes and a wave stay in registers; a workgroup goes once through LDS (two
-// buffers in turn, so one barrier per sum is enough).
+// buffers in turn, so one barrier per sum is enough): every 16 lanes take the 16 places of its
+// waves, those of waves that it has not are 0.
 template <int TPR, int NS>
 __device__ __forceinline__ void row_sum(float (&v)[NS], float (*sh)[16][2], int& turn) {
 #pragma unroll
   for (int k = 0; k < NS; ++k) {
-    v[k] += mov_dpp_f32<0xB1>(v[k]);
-    v[k] += mov_dpp_f32<0x4E>(v[k]);
-    v[k] += mov_dpp_f32<0x141>(v[k]);
-    v[k] += mov_dpp_f32<0x140>(v[k]);
+    v[k] = sum16(v[k]);
     if constexpr (TPR >= 64)
       v[k] = ((readlane_f(v[k], 0) + readlane_f(v[k], 16)) + readlane_f(v[k], 32)) +
              readlane_f(v[k], 48);
@@ -156,74 +168,110 @@ __device__ __forceinline__ void row_sum(float (&v)[NS], float (*sh)[16][2], int&
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < NS; ++k) {
-      float s = b[0][k];
-      for (int w = 1; w < (int)blockDim.x / 64; ++w) s += b[w][k];
-      v[k] = s;
-    }
+    for (int k = 0; k < NS; ++k) v[k] = sum16(b[threadIdx.x & 15][k]);
   }
+}
+
+// The thread's sum of its own values f, or of their squares about c.
+template <bool SQUARES, int TPR, int NIT, int V>
+__device__ __forceinline__ float own_sum(const Cols<TPR, NIT, V>& C, bool whole,
+                                         const float (&f)[NIT][V], float c) {
+  float s = 0.f;
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < NIT; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float d = f[i][k] - c;
+        s = SQUARES ? fmaf(d, d, s) : s + f[i][k];
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NIT; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float d = C.own(i, k) ? (SQUARES ? f[i][k] - c : f[i][k]) : 0.f;
+        s = SQUARES ? fmaf(d, d, s) : s + d;
+      }
+  }
+  return s;
 }
 
 // mean and 1 / sqrt(var + eps) (0 and 1 / rms) of the row's values f.  LayerNorm in a workgroup:
 // each wave sums its values, then their squares about its own mean, and the waves' pairs are put
 // together about the row's mean (one barrier instead of two, and no difference of large sums).
+// share: the number of values of each wave, mine: 1 / this wave's (1 / D where a wave has a row).
 template <int TPR, int NIT, int V>
-__device__ __forceinline__ void row_stats(const Cols<TPR, NIT, V>& C, const float (&f)[NIT][V],
-                                          float inv, bool layer, float eps, float (*sh)[16][2],
+__device__ __forceinline__ void row_stats(const Cols<TPR, NIT, V>& C, bool whole,
+                                          const float (&f)[NIT][V], float inv, float mine,
+                                          bool layer, float eps, float (*sh)[16][2],
                                           const float* share, int& turn, float& mean, float& rho) {
   mean = 0.f;
-  float s[1] = {0.f}, count = 0.f;
+  float s[1];
   int none = 0;
   if (layer) {
-#pragma unroll
-    for (int i = 0; i < NIT; ++i)
-#pragma unroll
-      for (int k = 0; k < V; ++k) s[0] += C.own(i, k) ? f[i][k] : 0.f;
+    s[0] = own_sum<false>(C, whole, f, 0.f);
     row_sum<(TPR < 64 ? TPR : 64), 1>(s, sh, none);
-    if constexpr (TPR > 64) count = share[wave_id()];
-    mean = s[0] * (TPR > 64 ? (count > 0.f ? 1.f / count : 0.f) : inv);
+    mean = s[0] * mine;
   }
-  s[0] = 0.f;
-#pragma unroll
-  for (int i = 0; i < NIT; ++i)
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const float d = C.own(i, k) ? f[i][k] - mean : 0.f;
-      s[0] = fmaf(d, d, s[0]);
-    }
+  s[0] = own_sum<true>(C, whole, f, mean);
   if constexpr (TPR <= 64) {
     row_sum<TPR, 1>(s, sh, none);
   } else if (!layer) {
     row_sum<TPR, 1>(s, sh, turn);
   } else {
-    float w[1] = {s[0]};
-    row_sum<64, 1>(w, sh, none);
+    row_sum<64, 1>(s, sh, none);
     float(*b)[2] = sh[turn];
     turn ^= 1;
-    if (lane_id() == 0) b[wave_id()][0] = mean, b[wave_id()][1] = w[0];
+    if (lane_id() == 0) b[wave_id()][0] = mean, b[wave_id()][1] = s[0];
     __syncthreads();
-    const int waves = blockDim.x / 64;
-    mean = 0.f;
-    for (int q = 0; q < waves; ++q) mean = fmaf(b[q][0], share[q], mean);
-    mean *= inv;
-    s[0] = 0.f;
-    for (int q = 0; q < waves; ++q) {
-      const float d = b[q][0] - mean;
-      s[0] += fmaf(d * d, share[q], b[q][1]);
-    }
+    const int q = threadIdx.x & 15;
+    const float mq = b[q][0];
+    mean = sum16(mq * share[q]) * inv;
+    const float d = mq - mean;
+    s[0] = sum16(fmaf(d * d, share[q], b[q][1]));
   }
   rho = __builtin_amdgcn_rsqf(fmaf(s[0], inv, eps));
 }
 
-// the number of a row's values that each wave of the workgroup holds
+// The thread's sums of its own values q, and of q n.
 template <int TPR, int NIT, int V>
-__device__ __forceinline__ void wave_shares(const Cols<TPR, NIT, V>& C, float* share) {
+__device__ __forceinline__ void own_sums(const Cols<TPR, NIT, V>& C, bool whole,
+                                         const float (&q)[NIT][V], const float (&n)[NIT][V],
+                                         float (&sum)[2]) {
+  sum[0] = sum[1] = 0.f;
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < NIT; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        sum[0] += q[i][k];
+        sum[1] = fmaf(q[i][k], n[i][k], sum[1]);
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NIT; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float v = C.own(i, k) ? q[i][k] : 0.f;
+        sum[0] += v;
+        sum[1] = fmaf(v, n[i][k], sum[1]);
+      }
+  }
+}
+
+// The number of a row's values that each wave of the workgroup holds (0 for waves that it has not,
+// whose places in sh are cleared).
+template <int TPR, int NIT, int V>
+__device__ __forceinline__ void wave_shares(const Cols<TPR, NIT, V>& C, float* share,
+                                            float (*sh)[16][2]) {
   if constexpr (TPR > 64) {
+    if (threadIdx.x < 64) ((float*)sh)[threadIdx.x] = 0.f;
     if (threadIdx.x < 16) {
       int n = 0;
       for (int i = 0; i < NIT; ++i)
         n += max(0, min(64 * V, C.D - (i * (int)blockDim.x + (int)threadIdx.x * 64) * V));
-      share[threadIdx.x] = (float)n;
+      share[threadIdx.x] = threadIdx.x < blockDim.x / 64 ? (float)n : 0.f;
     }
     __syncthreads();
   }
@@ -254,7 +302,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const gnnea_
   const bool layer = a.kind == GNNEA_NORM_LAYER, wb = a.w_dtype == GNNEA_BF16;
   const float inv = 1.f / (float)a.D;
   __shared__ float share[16];
-  wave_shares(C, share);
+  wave_shares(C, share, sh);
+  const bool whole = C.whole();
+  const float mine = TPR > 64 ? (share[wave_id()] > 0.f ? 1.f / share[wave_id()] : 0.f) : inv;
   float P[NIT][V], Q[NIT][V], W[NIT][V], B[NIT][V];
   const int64_t step = (int64_t)gridDim.x * RPB;
   int64_t row = (int64_t)xcd_remap(blockIdx.x, gridDim.x) * RPB + threadIdx.x / TPR;
@@ -296,7 +346,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const gnnea_
     if (row + step < a.n) load(row + step);  // on its way while this row is computed
     float mean = 0.f, rho = 1.f, mean2 = 0.f, rho2 = 1.f;
     if constexpr (IN) {
-      if (a.post) row_stats(C, y, inv, layer, a.eps, sh, share, turn, mean, rho);
+      if (a.post) row_stats(C, whole, y, inv, mine, layer, a.eps, sh, share, turn, mean, rho);
 #pragma unroll
       for (int i = 0; i < NIT; ++i) {
 #pragma unroll
@@ -309,7 +359,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const gnnea_
       }
     }
     if (a.pre) {
-      row_stats(C, r, inv, layer, a.eps, sh, share, turn, mean2, rho2);
+      row_stats(C, whole, r, inv, mine, layer, a.eps, sh, share, turn, mean2, rho2);
 #pragma unroll
       for (int i = 0; i < NIT; ++i) {
         float h[V];
@@ -340,10 +390,15 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
   const Cols<TPR, NIT, V> C{a.D, (int)(threadIdx.x % (TPR < 256 ? TPR : 1024))};
   const bool layer = a.kind == GNNEA_NORM_LAYER, wb = a.w_dtype == GNNEA_BF16;
   const float inv = 1.f / (float)a.D;
+  const bool whole = C.whole();
   float P[NIT][V], Q[NIT][V], W[NIT][V], acc[kHeld][NIT][V];
   if constexpr (!kLds) {
 #pragma unroll
     for (int q = 0; q < kHeld; ++q) clear_row(acc[q]);
+  }
+  if constexpr (TPR > 64) {  // (places of waves that the workgroup has not: 0)
+    if (threadIdx.x < 64) ((float*)sh)[threadIdx.x] = 0.f;
+    __syncthreads();
   }
   // four values of a sum at a time, the threads' next to each other
   const int nt = blockDim.x;
@@ -423,7 +478,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
       unpack16(rm[i], m[i]);
     }
     if (kAhead && row + step < a.n) load(row + step);
-    float sum[2] = {0.f, 0.f};
+    float sum[2];
 #pragma unroll
     for (int i = 0; i < NIT; ++i) {
 #pragma unroll
@@ -442,12 +497,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         m[i][k] *= W[i][k];
-        const float q = C.own(i, k) ? m[i][k] : 0.f;
-        sum[0] += q;
-        sum[1] = fmaf(q, r[i][k], sum[1]);
       }
     }
     if (a.dh) {
+      own_sums(C, whole, m, r, sum);
       row_sum<TPR, 2>(sum, sh, turn);
       const float m0 = layer ? sum[0] * inv : 0.f, m1 = sum[1] * inv;
 #pragma unroll
@@ -456,7 +509,6 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
         for (int k = 0; k < V; ++k)
           d[i][k] = fmaf(st.w, m[i][k] - m0 - r[i][k] * m1, d[i][k]);
     }
-    sum[0] = sum[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < NIT; ++i) {
       if (a.dx) store_row<T>(C, (T*)a.dx + row * a.lddx, i, d[i]);
@@ -471,9 +523,6 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
             z[i][k] = dg[k] * g.rest * fmaf(n[i][k], P[i][k], Q[i][k]);
           }
           r[i][k] = dg[k] * P[i][k];
-          const float q = C.own(i, k) ? r[i][k] : 0.f;
-          sum[0] += q;
-          sum[1] = fmaf(q, n[i][k], sum[1]);
         }
         add(0, i, dg, n[i]);
         if constexpr (BIAS) add(1, i, dg, ones);
@@ -483,6 +532,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const gnnea_
     if (IN && a.dy) {
       float q0 = 0.f, q1 = 0.f;
       if (a.post) {
+        own_sums(C, whole, r, n, sum);
         row_sum<TPR, 2>(sum, sh, turn);
         q0 = layer ? sum[0] * inv : 0.f;
         q1 = sum[1] * inv;
