@@ -27,10 +27,10 @@
 // are full), and the next row is read while one is computed.  Per-row reads of the vectors and
 // element-wise tails had cost 1.9x: 1M rows of 300 fp32, training pass 5.08 ms, now 3.27.
 //
-// Measured: 1M x 300 fp32 with a full gate, forward 1.20 ms (6.0 GB, 5.0 TB/s), backward 2.03
-// (9.6 GB, 4.7 TB/s); 8191 x 4097 bf16 LayerNorm, forward 93 us, backward 123 (2.9, 3.3 TB/s: a
-// row's exchange between waves waits with nothing else to run); 30000 x 300 bf16 forward 22 us
-// (4.1 TB/s); 2000 x 300 7 + 10 + 5 us of launches.
+// Measured: 1M x 300 fp32 with a full gate, forward 1.20 ms (6.0 GB, 5.0 TB/s), backward 2.05
+// (9.6 GB, 4.7 TB/s); bf16 LayerNorm of 8191 rows, 4096 wide: forward 50 us, backward 89 (5.3 and
+// 4.5 TB/s), 4097 wide: 79 and 116 (a ninth wave for one value, and rows at odd addresses); 30000 x
+// 300 bf16 forward 22 us (4.1 TB/s); 2000 x 300 7 + 10 + 5 us of launches.
 //
 // Statistics, sums and gradients are fp32; the column sums go per thread over its rows, then over
 // the workgroup's rows, then over workgroups (fp64) in a fixed order: results do not change from

@@ -311,3 +311,31 @@ def test_offsets_past_32_bits(device):
     Qs, ks = kv[:, :16].detach().clone().requires_grad_(), q.clone().requires_grad_()
     want = torch.autograd.grad(dot_attention(small, Qs, ks, do, 2), (Qs, ks), kv[:, 16:].contiguous())
     assert torch.equal(got[1], want[1]) and torch.equal(got[0][cols.to(device)], want[0])
+
+
+@pytest.mark.parametrize("R,C", [(0, 4), (4, 0), (0, 0)])
+def test_no_rows_or_columns(device, R, C):
+    from gnnea.graph import DeviceCSR
+    none = torch.zeros(0, dtype=torch.int64, device=device)
+    adj = DeviceCSR.from_coo(none, none, None, R, C)
+    q, k = torch.ones(R, 8, device=device), torch.ones(C, 4, device=device)
+    out, dq, dk, dv = both(adj, q, k, k.clone(), torch.ones_like(q), 2, 1)
+    assert out.shape == dq.shape == (R, 8) and dk.shape == dv.shape == (C, 4)
+    assert not out.any() and not dq.any() and not dk.any() and not dv.any()
+
+
+def test_shared_leaves_and_frozen_inputs(device):
+    """One tensor as q, k and v gets the sum of the three gradients; without a gradient wanted the
+    outputs are the same bits."""
+    from gnnea.attention import dot_attention
+    mask, q, _, _, do = case(30, 30, 2, 2, 16, torch.float32, 5, device, 8)
+    adj = csr(device, mask)
+    x = q.clone().requires_grad_()
+    out = dot_attention(adj, x, x, x, 2)
+    got, = torch.autograd.grad(out, x, do)
+    parts = both(adj, q, q.clone(), q.clone(), do, 2, 2)
+    assert torch.equal(out.detach(), parts[0]) and torch.equal(out.detach(), dot_attention(adj, q, q, q, 2))
+    # the engine adds the three in an order of its own: two roundings of the sum
+    want = parts[1].double() + parts[2].double() + parts[3].double()
+    bound = 2 * U * (parts[1].abs() + parts[2].abs() + parts[3].abs()).double()
+    assert bool(((got.double() - want).abs() <= bound + 1e-37).all())

@@ -307,3 +307,16 @@ def test_offsets_past_32_bits(device):
     db, dy = torch.autograd.grad(r, (b, y), dr)
     assert bool((db == n).all())
     assert bool((dy[-70:].float().abs() <= 2.0 ** -8).all())  # a constant's gradient through N is 0
+
+
+def test_the_same_tensor_twice(device):
+    """residual_norm(x, x): the gradient is the sum of both arguments' gradients."""
+    from gnnea.norm import residual_norm
+    t, dr, dh = inputs(30, 300, torch.float32, torch.float32, "none", device, 11)
+    x = t["x"].clone().requires_grad_()
+    r, h = residual_norm(x, x, scale=0.5, kind="layer")
+    got, = torch.autograd.grad((r, h), x, (dr, dh))
+    a, b = (t["x"].clone().requires_grad_() for _ in range(2))
+    r2, h2 = residual_norm(a, b, scale=0.5, kind="layer")
+    ga, gb = torch.autograd.grad((r2, h2), (a, b), (dr, dh))
+    assert torch.equal(r, r2) and torch.equal(got, ga + gb)
