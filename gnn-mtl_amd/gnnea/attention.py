@@ -108,7 +108,7 @@ class DotAttentionFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         stat = torch.empty((q.shape[0], ctx.meta[0], 2), dtype=torch.float32, device=q.device)
-        a = _problem(ctx.csr, q, k, v, ctx.meta)
+        a = _problem(ctx.csr, q, k, v, ctx.meta)  # from what is saved, which hooks may have moved
         a.lse, a.stat = lse.data_ptr(), stat.data_ptr()
         a.dout, a.lddo = dout.data_ptr(), _ld(dout)
         a.dq, a.lddq = dq.data_ptr(), q.shape[1]

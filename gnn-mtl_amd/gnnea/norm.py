@@ -26,15 +26,10 @@ def _code(dtype):
 
 def _problem(x, y, gate, vecs, meta):
     kind, eps, post, pre, alpha = meta
-    scale, pw, pb, qw, qb = vecs
-    a = NormProblem()
-    a.n, a.D, a.dtype = x.shape[0], x.shape[1], _code(x.dtype)
-    w = next((v for v in vecs if v is not None), None)
-    if w is None and gate is not None and gate.dim() == 1:
-        w = gate
-    a.w_dtype = _code(w.dtype if w is not None else torch.float32)
-    a.kind, a.eps, a.post, a.pre, a.alpha = kind, eps, post, pre, alpha
-    a.x, a.ldx = x.data_ptr(), _ld(x)
+    n, D = x.shape
+    a = NormProblem(n=n, D=D, dtype=_code(x.dtype), kind=kind, eps=eps, post=post, pre=pre,
+                    alpha=alpha, x=x.data_ptr(), ldx=_ld(x))
+    w = None
     if y is not None:
         a.y, a.ldy = y.data_ptr(), _ld(y)
     if gate is not None:
@@ -42,12 +37,41 @@ def _problem(x, y, gate, vecs, meta):
         if gate.dim() == 2:
             a.gate_mode, a.ldg = _lib.GNNEA_GATE_FULL, _ld(gate)
         else:
-            a.gate_mode = _lib.GNNEA_GATE_ROW
-    for name, v in (("scale", scale), ("post_w", pw), ("post_b", pb), ("pre_w", qw),
-                    ("pre_b", qb)):
+            a.gate_mode, w = _lib.GNNEA_GATE_ROW, gate
+    for name, v in zip(_VECTORS, vecs):
         if v is not None:
             setattr(a, name, v.data_ptr())
+            w = v
+    a.w_dtype = _lib.GNNEA_F32 if w is None else _code(w.dtype)
     return a
+
+
+_VECTORS = ("scale", "post_w", "post_b", "pre_w", "pre_b")
+_GRADS = ("dscale", "dpost_w", "dpost_b", "dpre_w", "dpre_b")
+
+
+def _forward(x, y, gate, vecs, meta, want_stats):
+    """(r, h, the rows' statistics for a backward pass)."""
+    a = _problem(x, y, gate, vecs, meta)
+    (n, D), dtype, device = x.shape, x.dtype, x.device
+    r = h = stats = None
+    if y is not None:
+        r = torch.empty((n, D), dtype=dtype, device=device)
+        a.r, a.ldr = r.data_ptr(), D
+    if meta[3]:
+        h = torch.empty((n, D), dtype=dtype, device=device)
+        a.h, a.ldh = h.data_ptr(), D
+    if want_stats:
+        stats = torch.empty((n, 4), dtype=torch.float32, device=device)
+        a.stats = stats.data_ptr()
+    if n:
+        with _lib.on_device(device):
+            check(_lib.lib().gnnea_norm_fwd(a, stream_of(device)))
+    return r, h, stats
+
+
+def _grad_rows(t, dtype):
+    return t if t.dtype == dtype and t.is_contiguous() else _rows(t, dtype)
 
 
 class NormFn(torch.autograd.Function):
@@ -55,23 +79,10 @@ class NormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, y, gate, scale, pw, pb, qw, qb, meta):
-        a = _problem(x, y, gate, (scale, pw, pb, qw, qb), meta)
-        n, D = x.shape
-        r = torch.empty((n, D), dtype=x.dtype, device=x.device) if y is not None else None
-        h = torch.empty((n, D), dtype=x.dtype, device=x.device) if meta[3] else None
-        if r is not None:
-            a.r, a.ldr = r.data_ptr(), D
-        if h is not None:
-            a.h, a.ldh = h.data_ptr(), D
-        stats = None
-        if any(ctx.needs_input_grad):
-            stats = torch.empty((n, 4), dtype=torch.float32, device=x.device)
-            a.stats = stats.data_ptr()
-        if n:
-            with _lib.on_device(x.device):
-                check(_lib.lib().gnnea_norm_fwd(a, stream_of(x.device)))
+        vecs = (scale, pw, pb, qw, qb)
+        r, h, stats = _forward(x, y, gate, vecs, meta, any(ctx.needs_input_grad))
         ctx.save_for_backward(x, y, gate, scale, pw, pb, qw, qb, stats)
-        ctx.problem = a  # (the addresses of the saved tensors; the backward adds its own to a copy)
+        ctx.meta = meta
         ctx.set_materialize_grads(False)
         return r, h
 
@@ -81,39 +92,50 @@ class NormFn(torch.autograd.Function):
         x, y, gate, scale, pw, pb, qw, qb, stats = ctx.saved_tensors
         if dr is None and dh is None:
             return (None,) * 9
-        vecs = (scale, pw, pb, qw, qb)
-        n, D = x.shape
+        vecs, need = (scale, pw, pb, qw, qb), ctx.needs_input_grad
+        (n, D), dtype, device = x.shape, x.dtype, x.device
         if n == 0:
-            return tuple(torch.zeros_like(t) if t is not None and need else None for t, need in
-                         zip((x, y, gate) + vecs + (None,), ctx.needs_input_grad))
-        a = NormProblem.from_buffer_copy(ctx.problem)
+            return tuple(torch.zeros_like(t) if t is not None and want else None for t, want in
+                         zip((x, y, gate) + vecs + (None,), need))
+        # from what is saved, which hooks may have moved since
+        a = _problem(x, y, gate, vecs, ctx.meta)
+        a.stats = stats.data_ptr()
         if dr is not None:
-            dr = _rows(dr, x.dtype)
+            dr = _grad_rows(dr, dtype)
             a.dr, a.lddr = dr.data_ptr(), _ld(dr)
         if dh is not None:
-            dh = _rows(dh, x.dtype)
+            dh = _grad_rows(dh, dtype)
             a.dh, a.lddh = dh.data_ptr(), _ld(dh)
-        need = ctx.needs_input_grad
         out = [None] * 9
         a.lddx = a.lddy = a.lddg = D
-        for k, name in ((0, "dx"), (1, "dy"), (2, "dgate")):
-            if need[k] and (k < 2 or gate.dim() == 2):
-                out[k] = torch.empty((n, D), dtype=x.dtype, device=x.device)
-                setattr(a, name, out[k].data_ptr())
-        if need[2] and gate.dim() == 1:
-            out[2] = torch.empty_like(gate)
-            a.dgate = out[2].data_ptr()
-        for k, name in enumerate(("dscale", "dpost_w", "dpost_b", "dpre_w", "dpre_b")):
-            if need[3 + k]:
-                out[3 + k] = torch.empty_like(vecs[k])
-                setattr(a, name, out[3 + k].data_ptr())
+        if need[0]:
+            out[0] = t = torch.empty((n, D), dtype=dtype, device=device)
+            a.dx = t.data_ptr()
+        if need[1]:
+            out[1] = t = torch.empty((n, D), dtype=dtype, device=device)
+            a.dy = t.data_ptr()
+        sums = any(need[3:8])
+        if need[2]:
+            rows = gate.dim() == 2
+            out[2] = t = torch.empty((n, D), dtype=dtype, device=device) if rows else \
+                torch.empty_like(gate)
+            a.dgate = t.data_ptr()
+            sums = sums or not rows
         L = _lib.lib()
         ws, ws_bytes = None, 0
-        if any(need[3:8]) or (need[2] and gate.dim() == 1):
+        if sums:
+            # the vectors all have one type
+            wanted = [k for k in range(5) if need[3 + k]]
+            if wanted:
+                like = vecs[wanted[0]]
+                got = torch.empty((len(wanted), D), dtype=like.dtype, device=device).unbind(0)
+                for k, t in zip(wanted, got):
+                    out[3 + k] = t
+                    setattr(a, _GRADS[k], t.data_ptr())
             ws_bytes = int(L.gnnea_norm_bwd_ws_bytes(n, D, a.dtype))
-            ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=x.device)
-        with _lib.on_device(x.device):
-            check(L.gnnea_norm_bwd(a, ptr(ws), ws_bytes, stream_of(x.device)))
+            ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=device)
+        with _lib.on_device(device):
+            check(L.gnnea_norm_bwd(a, ptr(ws), ws_bytes, stream_of(device)))
         return tuple(out)
 
 
@@ -157,6 +179,13 @@ def _kind(kind, eps):
     return KINDS[kind]
 
 
+def _apply(x, y, gate, vecs, meta):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, y, gate) + tuple(vecs)):
+        return NormFn.apply(x, y, gate, *vecs, meta)
+    return _forward(x, y, gate, vecs, meta, False)[:2]
+
+
 def residual_norm(x, y, gate=None, scale=None, post_weight=None, post_bias=None, pre_weight=None,
                   pre_bias=None, kind="rms", eps=1e-6, post=True, pre=True):
     """(r, h): r = x + scale * sigmoid(gate) * N(y), h = N'(r).
@@ -188,7 +217,7 @@ def residual_norm(x, y, gate=None, scale=None, post_weight=None, post_bias=None,
                                           row_gate))
     if gate is not None:
         gate = row_gate if row_gate is not None else _matrix("gate", gate, x)
-    return NormFn.apply(_rows(x), y, gate, *vecs, (code, float(eps), int(post), int(pre), alpha))
+    return _apply(_rows(x), y, gate, vecs, (code, float(eps), int(post), int(pre), alpha))
 
 
 def norm(x, weight=None, bias=None, kind="rms", eps=1e-6):
@@ -197,5 +226,5 @@ def norm(x, weight=None, bias=None, kind="rms", eps=1e-6):
     _lib.require_device(x, weight, bias)
     code = _kind(kind, eps)
     weight, bias = _vectors(x, ("weight", "bias"), (weight, bias))
-    return NormFn.apply(_rows(x), None, None, None, None, None, weight, bias,
-                        (code, float(eps), 0, 1, 1.0))[1]
+    return _apply(_rows(x), None, None, (None, None, None, weight, bias),
+                  (code, float(eps), 0, 1, 1.0))[1]

@@ -339,3 +339,19 @@ def test_shared_leaves_and_frozen_inputs(device):
     want = parts[1].double() + parts[2].double() + parts[3].double()
     bound = 2 * U * (parts[1].abs() + parts[2].abs() + parts[3].abs()).double()
     assert bool(((got.double() - want).abs() <= bound + 1e-37).all())
+
+
+def test_saved_tensors_that_move(device):
+    """Saved tensors packed to the host and back (other addresses, other strides): the same bits."""
+    from gnnea.attention import dot_attention
+    mask, q, k, v, do = case(40, 40, 4, 2, 24, torch.float32, 6, device, 12, fused=True)
+    adj = csr(device, mask)
+    want = both(adj, q, k, v, do, 4, 2)
+    x = [t.detach().requires_grad_() for t in (q, k, v)]
+    with torch.autograd.graph.save_on_cpu():
+        out = dot_attention(adj, *x, 4, 2)
+    junk = [torch.full((40, 192), 7.0, device=device) for _ in range(8)]
+    got = torch.autograd.grad(out, x, do)
+    del junk
+    for a, b in zip(want[1:], got):
+        assert torch.equal(a, b)

@@ -320,3 +320,21 @@ def test_the_same_tensor_twice(device):
     r2, h2 = residual_norm(a, b, scale=0.5, kind="layer")
     ga, gb = torch.autograd.grad((r2, h2), (a, b), (dr, dh))
     assert torch.equal(r, r2) and torch.equal(got, ga + gb)
+
+
+def test_saved_tensors_that_move(device):
+    """Saved tensors packed to the host and back (other addresses, other strides): the same bits."""
+    from gnnea.norm import residual_norm
+    t, dr, dh = inputs(40, 60, torch.float32, torch.float32, "full", device, 13)
+    wide = torch.zeros(40, 200, device=device)
+    wide[:, 5:65] = t["x"]
+    t["x"] = wide[:, 5:65]
+    want = run(t, "layer", dr, dh)
+    leaf = {k: v.detach().requires_grad_() for k, v in t.items()}
+    with torch.autograd.graph.save_on_cpu():
+        r, h = residual_norm(*(leaf[k] for k in NAMES), kind="layer")
+    junk = [torch.full((40, 60), 7.0, device=device) for _ in range(8)]
+    got = torch.autograd.grad((r, h), [leaf[k] for k in NAMES], (dr, dh))
+    del junk
+    for k, g in zip(NAMES, got):
+        assert torch.equal(g, want[k]), k
