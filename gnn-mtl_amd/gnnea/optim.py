@@ -105,7 +105,11 @@ class AdamW(torch.optim.Optimizer):
         """g with p's order of elements (torch has seen to it that shapes and devices agree)."""
         if g.is_sparse or g.dtype != p.dtype or g.numel() != n or p.numel() != n:
             raise ValueError("gnnea.AdamW: gradients must be dense and like their parameter")
-        if (g.is_contiguous() and p.is_contiguous()) or g.stride() == p.stride():
+        if p.is_contiguous():
+            return g if g.is_contiguous() else g.contiguous()
+        if not _dense(p):
+            raise ValueError("gnnea.AdamW: parameters must be dense and without gaps")
+        if g.stride() == p.stride():
             return g
         return torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
 
@@ -129,17 +133,20 @@ class AdamW(torch.optim.Optimizer):
                 if device is None:
                     _lib.require_device(p)
                     device = p.device
+                if p.device != device:
+                    raise ValueError("gnnea.AdamW: parameters on more than one device")
                 if s is None:
                     fresh.append((i, p, g))
                     continue
+                if s["exp_avg"].device != device:
+                    raise ValueError("gnnea.AdamW: a parameter was moved to %s, its state is on %s"
+                                     % (device, s["exp_avg"].device))
                 row = self._state_row(s)
                 g = self._gradient(p, g, row[3])
                 held.append(g)
                 lists.setdefault(p.dtype, []).append((p.data_ptr(), g.data_ptr()) + row
                                                      + (base + i,))
             for i, p, g in fresh:
-                if p.device != device:
-                    raise ValueError("gnnea.AdamW: parameters on more than one device")
                 if step is None:
                     step = torch.zeros(1, dtype=torch.int64, device=device)
                 g = self._gradient(p, g, p.numel())

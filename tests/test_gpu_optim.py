@@ -376,3 +376,27 @@ def test_copies_duplicates_and_rates(device):
     opt.load_state_dict(copy.deepcopy(twin.state_dict()))
     assert where == (opt.state[p]["exp_avg"].data_ptr(), opt.state[p]["step"].data_ptr())
     assert int(opt.state[p]["step"]) == 2
+
+
+def test_parameters_that_were_moved(device):
+    """A parameter taken to the host, or replaced by a view with gaps, after its first step: refused
+    before any launch."""
+    from gnnea import GnneaError
+    from gnnea.optim import AdamW
+    ps = [torch.nn.Parameter(torch.ones(6, 4, device=device)) for _ in range(2)]
+    opt = AdamW(ps)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    ps[1].data = torch.ones(6, 8, device=device)[:, :4]
+    ps[1].grad = torch.ones(6, 4, device=device)
+    with pytest.raises(ValueError):
+        opt.step()
+    ps[1].grad = None
+    ps[1].data = torch.ones(6, 4)
+    ps[1].grad = torch.ones(6, 4)
+    with pytest.raises(ValueError):
+        opt.step()
+    ps[0].grad = None
+    with pytest.raises((GnneaError, ValueError)):
+        opt.step()
