@@ -41,6 +41,8 @@ class _Pieces:
             self.items = torch.stack([row, beg, stop, slot], 1).to(torch.int32).contiguous()
             self.rows = rows.to(torch.int32)
             self.ptr = torch.cat([end.new_zeros(1), end]).to(torch.int32)
+            # kept with the matrix, so the next call may come on another stream
+            torch.cuda.current_stream(csr.device).synchronize()
 
 
 def _pieces(csr):

@@ -225,6 +225,26 @@ def test_other_stream_and_partial_gradients(device):
     assert torch.equal(torch.autograd.grad(out, v2, do)[0], want[3])
 
 
+def test_first_calls_on_two_streams(device):
+    """What is kept with a matrix is written before the call that makes it returns."""
+    from gnnea.attention import _pieces
+    mask, q, k, v, do = case(40, 3000, 2, 1, 16, torch.float32, 3, device, 4)
+    adj, again = csr(device, mask), csr(device, mask)
+    want = both(csr(device, mask), q, k, v, do, 2, 1)
+    torch.cuda.synchronize()
+    pieces = _pieces(adj)
+    assert torch.cuda.current_stream(device).query() and pieces.n_long
+    streams = [torch.cuda.Stream(device) for _ in range(2)]
+    got = []
+    for s in streams:  # the second does not wait for the first
+        with torch.cuda.stream(s):
+            got.append(both(again, q, k, v, do, 2, 1))
+    torch.cuda.synchronize()
+    for g in got:
+        for a, b in zip(want, g):
+            assert torch.equal(a, b)
+
+
 def test_captured_and_replayed(device):
     """Two graphs of one matrix, replayed in turn with eager work between: both read new inputs."""
     from gnnea.attention import dot_attention
