@@ -43,15 +43,6 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                  state_bits=32, max_norm=None, seed=0):
-        if isinstance(lr, torch.Tensor):
-            if lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
-                raise ValueError("gnnea.AdamW: a tensor lr must be one fp32 value on the device")
-        elif not lr >= 0:
-            raise ValueError("gnnea.AdamW: lr must not be negative (got %r)" % (lr,))
-        if not eps > 0 or not weight_decay >= 0:
-            raise ValueError("gnnea.AdamW: eps must be positive and weight_decay not negative")
-        if len(betas) != 2 or not all(0 <= b < 1 for b in betas):
-            raise ValueError("gnnea.AdamW: betas must be in [0, 1) (got %r)" % (betas,))
         if state_bits not in (8, 32):
             raise ValueError("gnnea.AdamW: state_bits must be 8 or 32 (got %r)" % (state_bits,))
         if max_norm is not None and not max_norm > 0:
@@ -63,11 +54,35 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, group):
-        self._base.append(sum(len(g["params"]) for g in self.param_groups))
+        base = sum(len(g["params"]) for g in self.param_groups)
         super().add_param_group(group)
-        if len(set(map(id, self.param_groups[-1]["params"]))) != len(self.param_groups[-1]["params"]):
+        self._base.append(base)
+        try:
+            self._check_group(self.param_groups[-1])
+        except (TypeError, ValueError):
+            self.param_groups.pop()
+            self._base.pop()
+            raise
+
+    @staticmethod
+    def _check_lr(lr):
+        if isinstance(lr, torch.Tensor):
+            if lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
+                raise ValueError("gnnea.AdamW: a tensor lr must be one fp32 value on the device")
+        elif not lr >= 0:
+            raise ValueError("gnnea.AdamW: lr must not be negative (got %r)" % (lr,))
+
+    @classmethod
+    def _check_group(cls, group):
+        cls._check_lr(group["lr"])
+        eps, weight_decay, betas = group["eps"], group["weight_decay"], group["betas"]
+        if not eps > 0 or not weight_decay >= 0:
+            raise ValueError("gnnea.AdamW: eps must be positive and weight_decay not negative")
+        if len(betas) != 2 or not all(0 <= b < 1 for b in betas):
+            raise ValueError("gnnea.AdamW: betas must be in [0, 1) (got %r)" % (betas,))
+        if len(set(map(id, group["params"]))) != len(group["params"]):
             raise ValueError("gnnea.AdamW: a parameter is in its group twice")
-        for p in self.param_groups[-1]["params"]:
+        for p in group["params"]:
             if p.dtype not in FEATURE_DTYPES:
                 raise TypeError("gnnea.AdamW: fp32 or bf16 parameters required (got %s)" % p.dtype)
             if p.is_sparse or not _dense(p):
@@ -156,6 +171,11 @@ class AdamW(torch.optim.Optimizer):
                                                      + self._state_row(state[p]) + (base + i,))
             if not lists:
                 continue
+            lr = group["lr"]  # may have been replaced since the group was checked
+            self._check_lr(lr)
+            if isinstance(lr, torch.Tensor) and lr.device != device:
+                raise ValueError("gnnea.AdamW: lr is on %s, the parameters on %s"
+                                 % (lr.device, device))
             arrays = []
             for dtype, rows in lists.items():
                 table = np.array(rows, dtype=np.int64)
@@ -182,9 +202,6 @@ class AdamW(torch.optim.Optimizer):
             for group, step, arrays in groups:
                 lr, (b1, b2) = group["lr"], group["betas"]
                 on_device = isinstance(lr, torch.Tensor)
-                if on_device and lr.device != device:
-                    raise ValueError("gnnea.AdamW: lr is on %s, the parameters on %s"
-                                     % (lr.device, device))
                 ctl = torch.empty(_lib.GNNEA_ADAMW_CTL_BYTES // 4, dtype=torch.float32,
                                   device=device)
                 check(L.gnnea_adamw_begin(ptr(parts), n_parts, self.max_norm or 0.0, b1, b2,

@@ -400,3 +400,19 @@ def test_parameters_that_were_moved(device):
     ps[0].grad = None
     with pytest.raises((GnneaError, ValueError)):
         opt.step()
+
+
+def test_a_rate_that_was_replaced(device):
+    """A rate set after the group was made is checked at the step, before any launch."""
+    from gnnea.optim import AdamW
+    p, q = (torch.nn.Parameter(torch.ones(5, device=device)) for _ in range(2))
+    opt = AdamW([dict(params=[p]), dict(params=[q])], lr=torch.full((1,), 0.1, device=device))
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    opt.step()
+    was = p.detach().clone(), int(opt.state[p]["step"])
+    for lr in (torch.ones(1, device=device, dtype=torch.float64), torch.ones(1), -0.5,
+               torch.ones(2, device=device)):
+        opt.param_groups[1]["lr"] = lr
+        with pytest.raises(ValueError):
+            opt.step()
+        assert torch.equal(p, was[0]) and int(opt.state[p]["step"]) == was[1]

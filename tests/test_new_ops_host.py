@@ -152,6 +152,28 @@ def test_host_tensors_are_refused():
         AdamW([p]).step()
 
 
+@pytest.mark.parametrize("option", [dict(lr=-1.0), dict(lr=torch.ones(1)), dict(eps=0.0),
+                                    dict(weight_decay=-1e-3), dict(betas=(0.9, 1.0)),
+                                    dict(betas=(0.9,))])
+def test_adamw_options_of_a_group(option):
+    """A group's own options are held to the same rules, and a refused group leaves no trace."""
+    from gnnea.optim import AdamW
+    p, q, r = (torch.nn.Parameter(torch.zeros(3)) for _ in range(3))
+    with pytest.raises(ValueError):
+        AdamW([dict(params=[p], **option)])
+    with pytest.raises(ValueError):
+        AdamW([p], **option)
+    opt = AdamW([p, q])
+    for bad in (dict(params=[r], **option), dict(params=[p, r])):  # the second: p is there already
+        with pytest.raises(ValueError):
+            opt.add_param_group(bad)
+        assert len(opt.param_groups) == 1 and opt._base == [0]
+    with pytest.raises(TypeError):
+        opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(3).double())]))
+    opt.add_param_group(dict(params=[r]))
+    assert opt._base == [0, 2]
+
+
 def encoder_args(**kw):
     import types
     a = dict(num_layers=3, dim=12, feat_dim=12, act="relu", dropout=0.0, bias=1, n_heads=4,
