@@ -4,11 +4,18 @@
 //
 //   s_ic = scale q_i . k_c,  p = exp(s - L_i),  L_i = log sum_c exp(s_ic),  o_i = sum_c p v_c
 //   dp_ic = do_i . v_c,  delta_i = sum_c p dp,  ds = p (dp - delta)
-//   dq_i = scale (sum p dp k - delta sum p k)          rows of the matrix, one pass over k, v
+//   dq_i = scale (sum p (dp - c) k - e sum p k),  e = sum p (dp - c),  delta = c + e
+//                                                      rows of the matrix, one pass over k, v
 //   dk_c = scale sum_i ds q_i,  dv_c = sum_i p do_i    rows of its transpose, one pass over q, do
 //
 // The forward keeps a running maximum and sum (online softmax) and stores L; nothing per entry is
-// ever stored.  The row pass needs no o: delta falls out of the same pass (sum p dp), in fp32.
+// ever stored.  The row pass needs no o: delta falls out of the same pass, in fp32.
+//
+// c: the dp of one of the row's entries.  What all dp of a row have in common passes no gradient,
+// but summed into both terms of dq it would leave their rounding; less c, a row of one entry, or
+// of equal values, gives 0 exactly (and so do its terms of dk, whose ds subtracts the same dp).
+// A c far from the others would do harm of its own, so it moves to an entry of over 64 times the
+// weight of its own: p |c| then stays within 64 times the largest p |dp| met.
 //
 // A head's row of d_head values is held by LPH lanes, NCH 16-B chunks each; a wave has 64 / LPH
 // such groups, which take different heads of the same entry first (their reads are neighbours in
@@ -367,13 +374,15 @@ __global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, const Att
   const float factor = a.scale * kLog2e;
   const float lse = on ? a.lse[(int64_t)u.row * a.heads + head] : -INFINITY;
   uint4 q[NCH], d[NCH];
-  float A[NCH][V], B[NCH][V], delta;
+  // ref: c, the same in all groups of a head, of an entry of weight cap / 64; P: sum p, e: sum p (dp -
+  // c), A: sum p (dp - c) k, B: sum p k
+  float A[NCH][V], B[NCH][V], ref, cap, P, e;
   for (bool care = false;; care = true) {
     ColBatch cb(a, u);
     RowOffset off(a.n_cols, a.ldk);
     L.load_own((const T*)a.q + u.row * a.ldq + (int64_t)head * dh, on, q);
     L.load_own((const T*)a.dout + u.row * a.lddo + (int64_t)head * dh, on, d);
-    delta = 0.f;
+    ref = cap = P = e = 0.f;
     clear(A);
     clear(B);
     for (uint32_t done = 0; done < (uint32_t)cb.total; done += 64) {
@@ -384,10 +393,10 @@ __global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, const Att
         bool ok[U];
 #pragma unroll
         for (int s = 0; s < U; ++s) {
-          const int e = b + s * eps + slot;
+          const int i = b + s * eps + slot;
           // a row whose scores are all -inf has no weights (lse = -inf), like one without entries
-          ok[s] = lse != -INFINITY && e < cb.left;
-          const uint64_t j = off.of(min(e, 63));
+          ok[s] = lse != -INFINITY && i < cb.left;
+          const uint64_t j = off.of(min(i, 63));
 #pragma unroll
           for (int c = 0; c < NCH; ++c) rk[s][c] = L.raw(K + j, c);
 #pragma unroll
@@ -402,25 +411,51 @@ __global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, const Att
               rv[s][c] = L.mask(rv[s][c], c, ok[s]);
             }
         }
+        float p[U], y[U], most = 0.f;
 #pragma unroll
         for (int s = 0; s < U; ++s) {
-          const float x = head_dot<V, LPH>(q, rk[s]), y = head_dot<V, LPH>(d, rv[s]);
-          const float p = ok[s] ? __builtin_amdgcn_exp2f(fmaf(x, factor, -lse)) : 0.f;
-          const float pd = p * y;
-          delta += pd;
+          const float x = head_dot<V, LPH>(q, rk[s]);
+          y[s] = head_dot<V, LPH>(d, rv[s]);
+          p[s] = ok[s] ? __builtin_amdgcn_exp2f(fmaf(x, factor, -lse)) : 0.f;
+          most = fmaxf(most, p[s]);
+        }
+        if (__any(most > cap)) {
+          float to = y[0];
+          most = p[0];
+#pragma unroll
+          for (int s = 1; s < U; ++s)
+            if (p[s] > most) most = p[s], to = y[s];
+          for (int w = LPH << S.hs; w < 64; w <<= 1) {
+            const float mo = lane_xor(most, w), yo = lane_xor(to, w);
+            if (mo > most || (mo == most && yo < to)) most = mo, to = yo;
+          }
+          const float by = most > cap ? ref - to : 0.f;
+          if (most > cap) ref = to, cap = 64.f * most;
+          e = fmaf(by, P, e);
+#pragma unroll
+          for (int c = 0; c < NCH; ++c)
+#pragma unroll
+            for (int k = 0; k < V; ++k) A[c][k] = fmaf(by, B[c][k], A[c][k]);
+        }
+#pragma unroll
+        for (int s = 0; s < U; ++s) {
+          const float pd = p[s] * (y[s] - ref);
+          e += pd;
+          P += p[s];
 #pragma unroll
           for (int c = 0; c < NCH; ++c) {
             axpy<V>(pd, rk[s][c], A[c]);
-            axpy<V>(p, rk[s][c], B[c]);
+            axpy<V>(p[s], rk[s][c], B[c]);
           }
         }
       }
     }
-    const float z = on ? zero_of(A, zero_of(B, delta * 0.f)) : 0.f;
+    const float z = on ? zero_of(A, zero_of(B, e * 0.f)) : 0.f;
     if (care || !__any(z != z)) break;
   }
   for (int w = LPH << S.hs; w < 64; w <<= 1) {
-    delta += lane_xor(delta, w);
+    e += lane_xor(e, w);
+    if (u.slot >= 0) P += lane_xor(P, w);
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
@@ -431,19 +466,19 @@ __global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, const Att
   }
   if (slot != 0 || !on) return;
   if (u.slot >= 0) {
-    float* part = ws + ((int64_t)u.slot * a.heads + head) * (2 * dh + 1);
-    if (L.l == 0) part[0] = delta;
-    L.store(part + 1, A, 1.f);
-    L.store(part + 1 + dh, B, 1.f);
+    float* part = ws + ((int64_t)u.slot * a.heads + head) * (2 * dh + 4);
+    if (L.l == 0) part[0] = ref, part[1] = cap, part[2] = P, part[3] = e;
+    L.store(part + 4, A, 1.f);
+    L.store(part + 4 + dh, B, 1.f);
     return;
   }
 #pragma unroll
   for (int c = 0; c < NCH; ++c)
 #pragma unroll
-    for (int k = 0; k < V; ++k) A[c][k] = fmaf(-delta, B[c][k], A[c][k]);
+    for (int k = 0; k < V; ++k) A[c][k] = fmaf(-e, B[c][k], A[c][k]);
   L.store((T*)a.dq + u.row * a.lddq + (int64_t)head * dh, A, a.scale);
   if (L.l == 0)
-    *(float2*)(a.stat + 2 * ((int64_t)u.row * a.heads + head)) = make_float2(lse, delta);
+    *(float2*)(a.stat + 2 * ((int64_t)u.row * a.heads + head)) = make_float2(lse, ref + e);
 }
 
 // Columns: a row of the transposed matrix per wave; groups take key/value heads, then (entry,
@@ -538,7 +573,8 @@ __global__ __launch_bounds__(256) void k_attn_cols(const gnnea_attn a, const Att
 }
 
 // Joins the pieces of a long row: a workgroup per row and head.  Its waves take the pieces in turn,
-// four columns to a lane; their sums meet in LDS in wave order.
+// four columns to a lane; their sums meet in LDS in wave order.  The row pass's pieces are moved to
+// the c of the heaviest (equal ones: the smallest c, whatever the order).
 template <typename T>
 __global__ __launch_bounds__(512) void k_attn_join(const gnnea_attn a, int pass,
                                                    const float* __restrict__ ws) {
@@ -547,7 +583,7 @@ __global__ __launch_bounds__(512) void k_attn_join(const gnnea_attn a, int pass,
   const int s0 = a.long_ptr[w], n = a.long_ptr[w + 1] - s0;
   const bool fwd = pass == GNNEA_ATTN_FWD, rows = pass == GNNEA_ATTN_BWD_ROWS;
   const int heads = pass == GNNEA_ATTN_BWD_COLS ? a.kv_heads : a.heads;
-  const int wide = fwd ? dh + 2 : rows ? 2 * dh + 1 : 2 * dh;
+  const int wide = fwd ? dh + 2 : rows ? 2 * dh + 4 : 2 * dh;
   const float* part = ws + ((int64_t)s0 * heads + h) * wide;
   const int64_t step = (int64_t)heads * wide;
   const int lane = lane_id(), wv = wave_id();
@@ -563,17 +599,35 @@ __global__ __launch_bounds__(512) void k_attn_join(const gnnea_attn a, int pass,
       m = x > m || x != x ? x : m;
     }
   }
-  const float ref = m == -INFINITY ? 0.f : m;
+  float ref = m == -INFINITY ? 0.f : m;
+  if (rows) {
+    float top = -INFINITY;
+    for (int s = lane; s < n; s += 64) {
+      const float x = part[s * step], t = part[s * step + 1];
+      if (t > top || (t == top && x < ref)) top = t, ref = x;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const float x = __shfl_xor(ref, o, 64), t = __shfl_xor(top, o, 64);
+      if (t > top || (t == top && x < ref)) top = t, ref = x;
+    }
+  }
   // what a lane adds up: values lane, lane + 64, ... of a piece after its first words
-  const int skip = fwd ? 2 : rows ? 1 : 0, width = wide - skip;
+  const int skip = fwd ? 2 : rows ? 4 : 0, width = wide - skip;
   float one = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int s = wv; s < n; s += 8) {
     const float* p = part + s * step;
-    const float f = fwd ? __builtin_amdgcn_exp2f(p[0] - ref) : 1.f;
-    if (skip) one = fmaf(p[skip - 1], f, one);
+    const float f = fwd ? __builtin_amdgcn_exp2f(p[0] - ref) : 1.f, by = rows ? p[0] - ref : 0.f;
+    if (fwd) one = fmaf(p[1], f, one);
+    if (rows) one += fmaf(by, p[2], p[3]);
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-      if (c * 64 + lane < width) acc[c] = fmaf(p[skip + c * 64 + lane], f, acc[c]);
+    for (int c = 0; c < 8; ++c) {
+      const int at = c * 64 + lane;
+      if (at >= width) continue;
+      float x = p[skip + at];
+      if (rows && at < dh) x = fmaf(by, p[skip + dh + at], x);
+      acc[c] = fmaf(x, f, acc[c]);
+    }
   }
 #pragma unroll
   for (int c = 0; c < 8; ++c)
@@ -605,7 +659,7 @@ __global__ __launch_bounds__(512) void k_attn_join(const gnnea_attn a, int pass,
     a.lse[(int64_t)row * a.heads + h] = one == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(one);
   if (rows)
     *(float2*)(a.stat + 2 * ((int64_t)row * a.heads + h)) =
-        make_float2(a.lse[(int64_t)row * a.heads + h], one);
+        make_float2(a.lse[(int64_t)row * a.heads + h], ref + one);
 }
 
 static int attn_check(const gnnea_attn* a, int pass) {
@@ -695,7 +749,7 @@ static void attn_dispatch(const gnnea_attn& a, int pass, float* ws, hipStream_t 
 static int64_t attn_ws(const gnnea_attn* a, int pass) {
   const int64_t dh = a->d_head;
   if (pass == GNNEA_ATTN_FWD) return (int64_t)a->n_items * a->heads * (dh + 2) * 4;
-  if (pass == GNNEA_ATTN_BWD_ROWS) return (int64_t)a->n_items * a->heads * (2 * dh + 1) * 4;
+  if (pass == GNNEA_ATTN_BWD_ROWS) return (int64_t)a->n_items * a->heads * (2 * dh + 4) * 4;
   return (int64_t)a->n_items * a->kv_heads * 2 * dh * 4;
 }
 

@@ -945,8 +945,9 @@ int gnnea_adamw_moments(const gnnea_adamw_tensor* tensors, int32_t count, void* 
  * that no row has stored are never read.  heads % kv_heads == 0, d_head <= 256.  The matrix's
  * values are not used.
  * Backward, the probabilities recomputed from the scores and lse, dp = do . v:
- *   _bwd_rows  dq_i = scale (sum p dp k - delta sum p k), delta_i = sum p dp, over the matrix's
- *              rows; writes stat: n_rows x heads x {lse, delta} floats
+ *   _bwd_rows  dq_i = scale sum p (dp - delta) k, delta_i = sum p dp, over the matrix's rows (both
+ *              sums about the dp of one of the row's entries: 0 exactly where all its dp are equal);
+ *              writes stat: n_rows x heads x {lse, delta} floats
  *   _bwd_cols  dk, dv (summed over the heads that share a key/value head) over the transposed
  *              matrix's rows; reads stat
  * Rows of dq, dk, dv without entries are written with zeros.  Sums are fp32 in a fixed order.
