@@ -117,8 +117,12 @@ class AdamW(torch.optim.Optimizer):
 
     @staticmethod
     def _gradient(p, g, n):
-        """g with p's order of elements (torch has seen to it that shapes and devices agree)."""
-        if g.is_sparse or g.dtype != p.dtype or g.numel() != n or p.numel() != n:
+        """g with p's order of elements.  (torch compares the two where a gradient is assigned; the
+        parameter's data, type or place may have been replaced since.)"""
+        if p.dtype not in FEATURE_DTYPES:
+            raise TypeError("gnnea.AdamW: fp32 or bf16 parameters required (got %s)" % p.dtype)
+        if g.is_sparse or g.dtype != p.dtype or g.shape != p.shape or g.device != p.device or \
+                p.numel() != n:
             raise ValueError("gnnea.AdamW: gradients must be dense and like their parameter")
         if p.is_contiguous():
             return g if g.is_contiguous() else g.contiguous()
