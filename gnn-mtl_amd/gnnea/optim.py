@@ -25,6 +25,15 @@ def _dense(t):
     return True
 
 
+def _layout(t):
+    """(shape, strides) of a dense tensor: which element stands where.  Strides that mean nothing
+    (of dimensions of one element, of a tensor of none) are 0."""
+    shape = tuple(t.shape)
+    if 0 in shape:
+        return shape, (0,) * len(shape)
+    return shape, tuple(0 if n == 1 else st for n, st in zip(shape, t.stride()))
+
+
 class AdamW(torch.optim.Optimizer):
     """m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
     p = p (1 - lr weight_decay) - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps).
@@ -39,7 +48,10 @@ class AdamW(torch.optim.Optimizer):
                     clipping).  The norm is then in ``grad_norm`` (a device tensor), and a step
                     whose norm is not finite changes nothing; without it, such gradients reach
                     the parameters as in torch.
-    A parameter without a gradient is left as it is.  t counts the steps of a group."""
+    A parameter without a gradient is left as it is.  t counts the steps of a group.
+    Moments keep the order of memory that their parameter had when they were made: a parameter whose
+    shape, strides or device is another after that is refused.  A state dict names the order of 8-bit
+    codes ("layout"); without it they are taken as row-major."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                  state_bits=32, max_norm=None, seed=0):
@@ -50,6 +62,7 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.max_norm = state_bits, max_norm
         self.seed = int(seed) & 0xffffffff
         self.grad_norm = None
+        self._order = {}  # the layout that a parameter's moments have
         self._base = []  # number of a group's first parameter in the hash of the 8-bit rounding
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
@@ -90,13 +103,15 @@ class AdamW(torch.optim.Optimizer):
 
     def __getstate__(self):
         return dict(super().__getstate__(), state_bits=self.state_bits, max_norm=self.max_norm,
-                    seed=self.seed, grad_norm=None, _base=self._base)
+                    seed=self.seed, grad_norm=None, _base=self._base,
+                    _order=self._order)
 
     def _init_state(self, p, step):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("gnnea.AdamW: take one step before capturing (a captured first "
                                "step would set the moments to zero at every replay)")
         s = self.state[p]
+        self._order[p] = _layout(p)
         s["step"] = step
         if self.state_bits == 32:
             s["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
@@ -107,6 +122,17 @@ class AdamW(torch.optim.Optimizer):
             s["exp_avg_rms"] = torch.zeros(n, dtype=torch.uint8, device=p.device)
             # the exponents of m's and of sqrt(v)'s blocks (any valid one: every code is zero)
             s["scales"] = torch.full((2, -(-n // BLOCK)), 127, dtype=torch.uint8, device=p.device)
+
+    def _check_state(self, p, s):
+        if s["exp_avg"].device != p.device:
+            raise ValueError("gnnea.AdamW: a parameter was moved to %s, its state is on %s"
+                             % (p.device, s["exp_avg"].device))
+        order = self._order.get(p)
+        if order is None:
+            self._order[p] = _layout(p)
+        elif (order[0] != p.shape or order[1] != p.stride()) and order != _layout(p):
+            raise ValueError("gnnea.AdamW: a parameter's shape and strides were %s at its first step "
+                             "and are %s now" % (order, _layout(p)))
 
     def _state_row(self, s):
         """m, the second moment, the scales and the length of a state, for a descriptor."""
@@ -157,9 +183,7 @@ class AdamW(torch.optim.Optimizer):
                 if s is None:
                     fresh.append((i, p, g))
                     continue
-                if s["exp_avg"].device != device:
-                    raise ValueError("gnnea.AdamW: a parameter was moved to %s, its state is on %s"
-                                     % (device, s["exp_avg"].device))
+                self._check_state(p, s)
                 row = self._state_row(s)
                 g = self._gradient(p, g, row[3])
                 held.append(g)
@@ -233,6 +257,7 @@ class AdamW(torch.optim.Optimizer):
                 elif self.state_bits == 32:
                     out.append((s["exp_avg"], s["exp_avg_sq"]))
                 else:
+                    self._check_state(p, s)
                     m = torch.empty_like(p, dtype=torch.bfloat16)
                     u = torch.empty_like(p, dtype=torch.bfloat16)
                     rows.append((m.data_ptr(), u.data_ptr()) + self._state_row(s) + (0,))
@@ -245,6 +270,17 @@ class AdamW(torch.optim.Optimizer):
                                                      stream_of(device)))
         return out
 
+    def state_dict(self):
+        sd = super().state_dict()
+        if self.state_bits == 8:
+            state = sd["state"]
+            for saved, group in zip(sd["param_groups"], self.param_groups):
+                for key, p in zip(saved["params"], group["params"]):
+                    if key in state:
+                        state[key] = dict(state[key], layout=torch.tensor(
+                            self._order.get(p, _layout(p))))
+        return sd
+
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Takes the state as it is (codes stay uint8, moments of bf16 parameters stay fp32)."""
@@ -255,7 +291,7 @@ class AdamW(torch.optim.Optimizer):
         names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_rms",
                                                                         "scales")
         dtype = torch.float32 if self.state_bits == 32 else torch.uint8
-        new = {}
+        new, orders = {}, {}
         for old, group in zip(saved, self.param_groups):
             ps = dict(zip(old["params"], group["params"]))
             # (what is there is written into: a captured step keeps its addresses)
@@ -270,6 +306,17 @@ class AdamW(torch.optim.Optimizer):
                 shapes = dict(exp_avg=p.shape if self.state_bits == 32 else (n,),
                               exp_avg_sq=p.shape, exp_avg_rms=(n,), scales=(2, -(-n // BLOCK)))
                 have, s = self.state.get(p), dict(step=step)
+                order = _layout(p)
+                if self.state_bits == 8:
+                    was = got.get("layout")
+                    if torch.as_tensor(was).tolist() != list(map(list, order)) if was is not None \
+                            else not p.is_contiguous():
+                        raise ValueError("gnnea.AdamW: the codes of parameter %s are in the order %s, "
+                                         "the parameter in %s" % (key, "of rows" if was is None else
+                                                                  was, order))
+                if self._order.get(p) != order:
+                    have = None
+                orders[p] = order
                 for name in names:
                     t = got.get(name)
                     if t is None or t.dtype != dtype or tuple(t.shape) != tuple(shapes[name]):
@@ -291,3 +338,4 @@ class AdamW(torch.optim.Optimizer):
                     group[k] = float(v) if isinstance(v, torch.Tensor) else v
         self.state.clear()
         self.state.update(new)
+        self._order = orders

@@ -79,3 +79,80 @@ def test_gradients_that_are_not_the_parameters(lib):
     p.data = torch.zeros(6, 4)
     assert p.grad.shape == (4, 6)
     refused(lib, opt)
+
+
+def transposed(t):
+    return t.t().contiguous().t()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_order_that_changed(lib, bits):
+    """Moments belong to elements by the order of memory: a parameter of another order, or of
+    another shape of as many elements, is refused by step and by moments()."""
+    from gnnea.optim import AdamW
+    for new in (transposed(torch.ones(4, 6)), torch.ones(6, 4), torch.ones(24)):
+        p, q = parameters((3,), (4, 6))
+        opt = AdamW([p, q], state_bits=bits)
+        opt.step()
+        was = q.data
+        q.data, q.grad = new, torch.ones_like(new)
+        refused(lib, opt)
+        if bits == 8:
+            with pytest.raises(ValueError):
+                opt.moments()
+            assert not lib.count("gnnea_adamw_moments")
+        q.data, q.grad = was, torch.ones_like(was)
+        opt.step()
+    p, = parameters((1, 5))  # one row: its stride means nothing
+    opt = AdamW([p], state_bits=bits)
+    opt.step()
+    p.data = torch.zeros(5, 1).t()
+    p.grad = torch.ones(1, 5)
+    opt.step()
+
+
+def test_codes_are_saved_with_their_order(lib):
+    """8-bit codes lie flat in memory order, so a state dict names it: into a parameter of another
+    order they are refused; without a name they are row-major."""
+    import copy
+    from gnnea.optim import AdamW
+    row, = parameters((4, 6))
+    col = torch.nn.Parameter(transposed(torch.zeros(4, 6)))
+    col.grad = torch.ones_like(col)
+    one, two = AdamW([row], state_bits=8), AdamW([col], state_bits=8)
+    one.step()
+    two.step()
+    a, b = one.state_dict(), two.state_dict()
+    assert "layout" not in one.state[row]
+    for opt, other in ((one, b), (two, a)):
+        with pytest.raises(ValueError):
+            opt.load_state_dict(other)
+    one.load_state_dict(copy.deepcopy(a))
+    two.load_state_dict(copy.deepcopy(b))
+    for sd in (a, b):
+        sd["state"][0].pop("layout")
+    one.load_state_dict(a)
+    with pytest.raises(ValueError):
+        two.load_state_dict(b)
+    copy.deepcopy(one).step()
+    with pytest.raises(ValueError):  # (the codes' own order, not the one that the parameter has now)
+        row.data = transposed(row.data)
+        AdamW([row], state_bits=8).load_state_dict(one.state_dict())
+
+
+def test_32_bit_moments_follow_their_elements(lib):
+    """32-bit moments have their parameter's shape: loaded into another order, each goes to its own
+    element, also where the parameter's order changed after its first step."""
+    from gnnea.optim import AdamW
+    p, = parameters((4, 6))
+    opt = AdamW([p])
+    opt.step()
+    m = torch.arange(24.0).view(4, 6)
+    opt.state[p]["exp_avg"].copy_(m)
+    sd = opt.state_dict()
+    p.data, p.grad = transposed(p.data), None
+    opt.load_state_dict(sd)
+    s = opt.state[p]
+    assert torch.equal(s["exp_avg"], m) and s["exp_avg"].stride() == p.stride()
+    p.grad = torch.ones_like(p)
+    opt.step()
