@@ -281,61 +281,82 @@ class AdamW(torch.optim.Optimizer):
                             self._order.get(p, _layout(p))))
         return sd
 
+    def _loaded_options(self, old, group):
+        """The group's options as the saved ones would make them, checked."""
+        new = dict(group)
+        for k, v in old.items():
+            if k == "params":
+                continue
+            if isinstance(v, torch.Tensor):
+                if v.numel() != 1:
+                    raise ValueError("gnnea.AdamW: option %s must be one value (got %s)"
+                                     % (k, tuple(v.shape)))
+                v = float(v)
+            new[k] = v
+        self._check_group(new)
+        return new
+
+    def _loaded_state(self, key, p, got):
+        """(step, moments by name) of a saved state, checked against its parameter."""
+        if "step" not in got or torch.as_tensor(got["step"]).numel() != 1 or int(got["step"]) < 0:
+            raise ValueError("gnnea.AdamW: the state of parameter %s has no step" % (key,))
+        n, order = p.numel(), _layout(p)
+        if self.state_bits == 32:
+            shapes, dtype = dict(exp_avg=p.shape, exp_avg_sq=p.shape), torch.float32
+        else:
+            shapes = dict(exp_avg=(n,), exp_avg_rms=(n,), scales=(2, -(-n // BLOCK)))
+            dtype, was = torch.uint8, got.get("layout")
+            if torch.as_tensor(was).tolist() != list(map(list, order)) if was is not None \
+                    else not p.is_contiguous():
+                raise ValueError("gnnea.AdamW: the codes of parameter %s are in the order %s, the "
+                                 "parameter in %s" % (key, "of rows" if was is None else was, order))
+        for name, shape in shapes.items():
+            t = got.get(name)
+            if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape):
+                raise ValueError("gnnea.AdamW: %s of parameter %s must be %s %s for state_bits=%d"
+                                 % (name, key, tuple(shape), dtype, self.state_bits))
+        return int(got["step"]), {name: got[name] for name in shapes}
+
     @torch.no_grad()
     def load_state_dict(self, state_dict):
-        """Takes the state as it is (codes stay uint8, moments of bf16 parameters stay fp32)."""
+        """Takes the state as it is (codes stay uint8, moments of bf16 parameters stay fp32), all of
+        it or, where anything is refused, none."""
         saved = state_dict["param_groups"]
         if len(saved) != len(self.param_groups) or any(
                 len(a["params"]) != len(b["params"]) for a, b in zip(saved, self.param_groups)):
             raise ValueError("gnnea.AdamW: the loaded state has other parameter groups")
-        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_rms",
-                                                                        "scales")
-        dtype = torch.float32 if self.state_bits == 32 else torch.uint8
-        new, orders = {}, {}
+        plans = []
         for old, group in zip(saved, self.param_groups):
-            ps = dict(zip(old["params"], group["params"]))
-            # (what is there is written into: a captured step keeps its addresses)
+            options = self._loaded_options(old, group)
+            states = [(p, self._loaded_state(key, p, state_dict["state"][key]))
+                      for key, p in zip(old["params"], group["params"])
+                      if state_dict["state"].get(key)]
+            plans.append((group, options, states))
+        # memory for all of it; what is there is written into: a captured step keeps its addresses
+        new = {}
+        for group, _, states in plans:
             step = next((self.state[p]["step"] for p in group["params"] if p in self.state), None)
-            for key, p in ps.items():
-                got = state_dict["state"].get(key)
-                if not got:
-                    continue
-                t = torch.as_tensor(got["step"]).reshape(1).to(torch.int64)
-                step = t.to(p.device, copy=True) if step is None else step.copy_(t)
-                n = p.numel()
-                shapes = dict(exp_avg=p.shape if self.state_bits == 32 else (n,),
-                              exp_avg_sq=p.shape, exp_avg_rms=(n,), scales=(2, -(-n // BLOCK)))
-                have, s = self.state.get(p), dict(step=step)
-                order = _layout(p)
-                if self.state_bits == 8:
-                    was = got.get("layout")
-                    if torch.as_tensor(was).tolist() != list(map(list, order)) if was is not None \
-                            else not p.is_contiguous():
-                        raise ValueError("gnnea.AdamW: the codes of parameter %s are in the order %s, "
-                                         "the parameter in %s" % (key, "of rows" if was is None else
-                                                                  was, order))
-                if self._order.get(p) != order:
+            for p, (_, moments) in states:
+                if step is None or step.device != p.device:
+                    step = torch.zeros(1, dtype=torch.int64, device=p.device)
+                have = self.state.get(p)
+                if have is not None and (self._order.get(p) != _layout(p)
+                                         or have["exp_avg"].device != p.device):
                     have = None
-                orders[p] = order
-                for name in names:
-                    t = got.get(name)
-                    if t is None or t.dtype != dtype or tuple(t.shape) != tuple(shapes[name]):
-                        raise ValueError("gnnea.AdamW: %s of parameter %s must be %s %s for "
-                                         "state_bits=%d" % (name, key, tuple(shapes[name]), dtype,
-                                                            self.state_bits))
-                    if have is not None:
-                        s[name] = have[name]
-                    elif self.state_bits == 32:
-                        s[name] = torch.empty_like(p, dtype=dtype)
-                    else:
-                        s[name] = torch.empty(t.shape, dtype=dtype, device=p.device)
-                    s[name].copy_(t)
-                new[p] = s
-            for k, v in old.items():
-                if k == "lr" and isinstance(group["lr"], torch.Tensor):
-                    group["lr"].copy_(torch.as_tensor(v).reshape(group["lr"].shape))
-                elif k != "params":
-                    group[k] = float(v) if isinstance(v, torch.Tensor) else v
+                new[p] = s = dict(step=step)
+                for name, t in moments.items():
+                    s[name] = have[name] if have is not None else \
+                        torch.empty_like(p, dtype=t.dtype) if self.state_bits == 32 else \
+                        torch.empty(t.shape, dtype=t.dtype, device=p.device)
+        for group, options, states in plans:
+            for p, (step, moments) in states:
+                new[p]["step"].fill_(step)
+                for name, t in moments.items():
+                    new[p][name].copy_(t)
+            lr = group["lr"]
+            if isinstance(lr, torch.Tensor):
+                options["lr"] = lr if options["lr"] is lr else lr.fill_(options["lr"])
+            group.update(options)
         self.state.clear()
         self.state.update(new)
-        self._order = orders
+        self._order = {p: _layout(p) for p in new}

@@ -156,3 +156,76 @@ def test_32_bit_moments_follow_their_elements(lib):
     assert torch.equal(s["exp_avg"], m) and s["exp_avg"].stride() == p.stride()
     p.grad = torch.ones_like(p)
     opt.step()
+
+
+def snapshot(opt):
+    import copy
+    state = {p: {k: (v, v.clone()) for k, v in s.items()} for p, s in opt.state.items()}
+    groups = [{k: copy.deepcopy(v) for k, v in g.items() if k != "params"} for g in opt.param_groups]
+    return state, groups, dict(opt._order)
+
+
+def assert_unchanged(opt, was):
+    state, groups, order = was
+    assert set(opt.state) == set(state) and opt._order == order
+    for p, s in state.items():
+        assert set(opt.state[p]) == set(s)
+        for k, (same, value) in s.items():
+            assert opt.state[p][k] is same and torch.equal(same, value), k
+    for g, old in zip(opt.param_groups, groups):
+        assert {k: v for k, v in g.items() if k != "params"} == old
+
+
+def spoil(sd, how):
+    second, group = sd["state"][1], sd["param_groups"][1]
+    if how == "shape":
+        second["exp_avg"] = second["exp_avg"].reshape(-1)[:-1]
+    elif how == "type":
+        second["exp_avg"] = second["exp_avg"].double()
+    elif how == "name":
+        del second["exp_avg"]
+    elif how == "step":
+        del second["step"]
+    elif how == "steps":
+        second["step"] = torch.zeros(2)
+    elif how == "negative":
+        second["step"] = -1
+    elif how == "group":
+        sd["param_groups"].pop()
+    elif how == "betas":
+        group["betas"] = (0.9, 1.0)
+    elif how == "lr":
+        group["lr"] = -1.0
+    elif how == "lrs":
+        group["lr"] = torch.ones(2)
+    elif how == "eps":
+        group["eps"] = 0.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("how", ["shape", "type", "name", "step", "steps", "negative", "group",
+                                 "betas", "lr", "lrs", "eps", "bits"])
+def test_a_refused_load_changes_nothing(lib, bits, how):
+    """The first parameter's part of the dict is sound, and not taken: nor its step or options."""
+    import copy
+    from gnnea.optim import AdamW
+
+    def make(bits, lr):
+        ps = parameters((5,), (4, 6))
+        opt = AdamW([dict(params=[ps[0]]), dict(params=[ps[1]], lr=lr)], lr=lr, state_bits=bits)
+        opt.step()
+        for p in ps:
+            opt.state[p]["step"].fill_(round(lr * 1000))
+            opt.state[p]["exp_avg"].fill_(3)
+        return opt
+    live, other = make(bits, 0.005), make(8 if (how == "bits") == (bits == 32) else 32, 0.099)
+    sd = copy.deepcopy(other.state_dict())
+    spoil(sd, how)
+    was = snapshot(live)
+    with pytest.raises((ValueError, TypeError)):
+        live.load_state_dict(sd)
+    assert_unchanged(live, was)
+    live.step()
+    live.load_state_dict(make(bits, 0.099).state_dict())
+    assert int(live.state[live.param_groups[0]["params"][0]]["step"]) == 99
+    assert live.param_groups[1]["lr"] == 0.099
