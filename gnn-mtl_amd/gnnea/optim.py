@@ -93,6 +93,11 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("gnnea.AdamW: eps must be positive and weight_decay not negative")
         if len(betas) != 2 or not all(0 <= b < 1 for b in betas):
             raise ValueError("gnnea.AdamW: betas must be in [0, 1) (got %r)" % (betas,))
+        for name in ("amsgrad", "maximize", "differentiable"):
+            if group.get(name):
+                raise ValueError("gnnea.AdamW: %s is not done here" % name)
+        if weight_decay and not group.get("decoupled_weight_decay", True):
+            raise ValueError("gnnea.AdamW: weight_decay here is decoupled from the gradient")
         if len(set(map(id, group["params"]))) != len(group["params"]):
             raise ValueError("gnnea.AdamW: a parameter is in its group twice")
         for p in group["params"]:

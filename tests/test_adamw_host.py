@@ -229,3 +229,41 @@ def test_a_refused_load_changes_nothing(lib, bits, how):
     live.load_state_dict(make(bits, 0.099).state_dict())
     assert int(live.state[live.param_groups[0]["params"][0]]["step"]) == 99
     assert live.param_groups[1]["lr"] == 0.099
+
+
+@pytest.mark.parametrize("option,ok", [
+    (dict(maximize=True), False), (dict(amsgrad=True), False), (dict(differentiable=True), False),
+    (dict(decoupled_weight_decay=False, weight_decay=0.1), False),
+    (dict(decoupled_weight_decay=False, weight_decay=0.0), True),
+    (dict(maximize=False, amsgrad=False, foreach=True, initial_lr=0.1), True)])
+def test_options_that_the_step_does_not_do(lib, option, ok):
+    """torch's optimizers' options that would change the update are refused where they are on: in a
+    group, and in a state dict of torch's."""
+    from gnnea.optim import AdamW
+    p, = parameters((3,))
+    opt = AdamW([p])
+    sd = opt.state_dict()
+    sd["param_groups"][0].update(option)
+    if ok:
+        opt.load_state_dict(sd)
+        AdamW([dict(params=[p], **option)]).step()
+        return
+    with pytest.raises(ValueError):
+        opt.load_state_dict(sd)
+    assert not set(option) - {"weight_decay"} & set(opt.param_groups[0])
+    with pytest.raises(ValueError):
+        AdamW([dict(params=[p], **option)])
+
+
+def test_a_state_of_torchs(lib):
+    """torch.optim.Adam's and AdamW's own dicts, as they are by default."""
+    from gnnea.optim import AdamW
+    p, = parameters((3,))
+    for other in (torch.optim.Adam([p]), torch.optim.AdamW([p])):
+        other.step()
+        opt = AdamW([p])
+        opt.load_state_dict(other.state_dict())
+        assert torch.equal(opt.state[p]["exp_avg"], other.state[p]["exp_avg"])
+        assert int(opt.state[p]["step"]) == 1
+    with pytest.raises(ValueError):
+        AdamW([p]).load_state_dict(torch.optim.Adam([p], weight_decay=0.1).state_dict())
