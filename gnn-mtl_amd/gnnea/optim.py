@@ -48,7 +48,9 @@ class AdamW(torch.optim.Optimizer):
                     clipping).  The norm is then in ``grad_norm`` (a device tensor), and a step
                     whose norm is not finite changes nothing; without it, such gradients reach
                     the parameters as in torch.
-    A parameter without a gradient is left as it is.  t counts the steps of a group.
+    A parameter without a gradient is left as it is.  t counts a parameter's own steps, those with a
+    gradient, as in torch; parameters of a group with the same history share one counter (and one
+    small launch per step).
     Moments keep the order of memory that their parameter had when they were made: a parameter whose
     shape, strides or device is another after that is refused.  A state dict names the order of 8-bit
     codes ("layout"); without it they are taken as row-major."""
@@ -112,9 +114,6 @@ class AdamW(torch.optim.Optimizer):
                     _order=self._order)
 
     def _init_state(self, p, step):
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("gnnea.AdamW: take one step before capturing (a captured first "
-                               "step would set the moments to zero at every replay)")
         s = self.state[p]
         self._order[p] = _layout(p)
         s["step"] = step
@@ -127,6 +126,7 @@ class AdamW(torch.optim.Optimizer):
             s["exp_avg_rms"] = torch.zeros(n, dtype=torch.uint8, device=p.device)
             # the exponents of m's and of sqrt(v)'s blocks (any valid one: every code is zero)
             s["scales"] = torch.full((2, -(-n // BLOCK)), 127, dtype=torch.uint8, device=p.device)
+        return s
 
     def _check_state(self, p, s):
         if s["exp_avg"].device != p.device:
@@ -169,15 +169,22 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        groups, held, device = [], [], None
+        # everything is checked before anything is made or launched
+        todo, held, device = [], [], None
         state = self.state
         for base, group in zip(self._base, self.param_groups):
-            lists, step, fresh = {}, None, []
+            # by counter: [counter, rows by type, states without a gradient]; the parameters'
+            # first steps under None
+            counters = {}
             for i, p in enumerate(group["params"]):
-                s = state.get(p)
-                if s is not None and step is None:
+                s, g = state.get(p), p.grad
+                if s is not None:
                     step = s["step"]
-                g = p.grad
+                    c = counters.get(id(step))
+                    if c is None:
+                        c = counters[id(step)] = (step, {}, [])
+                    if g is None:
+                        c[2].append(s)
                 if g is None:
                     continue
                 if device is None:
@@ -186,36 +193,52 @@ class AdamW(torch.optim.Optimizer):
                 if p.device != device:
                     raise ValueError("gnnea.AdamW: parameters on more than one device")
                 if s is None:
-                    fresh.append((i, p, g))
-                    continue
-                self._check_state(p, s)
-                row = self._state_row(s)
-                g = self._gradient(p, g, row[3])
+                    c = counters.get(None)
+                    if c is None:
+                        c = counters[None] = (None, {}, [])
+                    g = self._gradient(p, g, p.numel())
+                    c[1].setdefault(p.dtype, []).append((p, g, base + i))
+                else:
+                    self._check_state(p, s)
+                    row = self._state_row(s)
+                    g = self._gradient(p, g, row[3])
+                    c[1].setdefault(p.dtype, []).append((p.data_ptr(), g.data_ptr()) + row
+                                                        + (base + i,))
                 held.append(g)
-                lists.setdefault(p.dtype, []).append((p.data_ptr(), g.data_ptr()) + row
-                                                     + (base + i,))
-            for i, p, g in fresh:
-                if step is None:
-                    step = torch.zeros(1, dtype=torch.int64, device=device)
-                g = self._gradient(p, g, p.numel())
-                held.append(g)
-                self._init_state(p, step)
-                lists.setdefault(p.dtype, []).append((p.data_ptr(), g.data_ptr())
-                                                     + self._state_row(state[p]) + (base + i,))
-            if not lists:
+            counters = [c for c in counters.values() if c[1]]
+            if not counters:
                 continue
             lr = group["lr"]  # may have been replaced since the group was checked
             self._check_lr(lr)
             if isinstance(lr, torch.Tensor) and lr.device != device:
                 raise ValueError("gnnea.AdamW: lr is on %s, the parameters on %s"
                                  % (lr.device, device))
-            arrays = []
-            for dtype, rows in lists.items():
-                table = np.array(rows, dtype=np.int64)
-                held.append(table)
-                arrays.append((table.ctypes.data, len(rows), _lib.GNNEA_BF16
-                               if dtype == torch.bfloat16 else _lib.GNNEA_F32))
-            groups.append((group, step, arrays))
+            todo.append((group, counters))
+        if any(step is None or idle for _, counters in todo for step, _, idle in counters) and \
+                torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("gnnea.AdamW: take a step with the same gradients before capturing "
+                               "(a captured first step would set the moments to zero, or a counter "
+                               "back, at every replay)")
+        groups = []
+        for group, counters in todo:
+            for step, lists, idle in counters:
+                if idle:
+                    kept = step.clone()
+                    for s in idle:
+                        s["step"] = kept
+                if step is None:
+                    step = torch.zeros(1, dtype=torch.int64, device=device)
+                    for rows in lists.values():
+                        rows[:] = [(p.data_ptr(), g.data_ptr())
+                                   + self._state_row(self._init_state(p, step)) + (index,)
+                                   for p, g, index in rows]
+                arrays = []
+                for dtype, rows in lists.items():
+                    table = np.array(rows, dtype=np.int64)
+                    held.append(table)
+                    arrays.append((table.ctypes.data, len(rows), _lib.GNNEA_BF16
+                                   if dtype == torch.bfloat16 else _lib.GNNEA_F32))
+                groups.append((group, step, arrays))
         if not groups:
             return loss
         L = _lib.lib()
@@ -340,15 +363,22 @@ class AdamW(torch.optim.Optimizer):
         # memory for all of it; what is there is written into: a captured step keeps its addresses
         new = {}
         for group, _, states in plans:
-            step = next((self.state[p]["step"] for p in group["params"] if p in self.state), None)
-            for p, (_, moments) in states:
-                if step is None or step.device != p.device:
-                    step = torch.zeros(1, dtype=torch.int64, device=p.device)
+            counter, of, to = {}, {}, {}  # p's counter; a counter's value; a value's counter
+            for p, (step, _) in states:
+                t = self.state[p]["step"] if p in self.state else None
+                if t is not None and t.device == p.device and of.setdefault(id(t), step) == step:
+                    counter[p] = t
+                    to.setdefault((step, p.device), t)
+            for p, (step, moments) in states:
+                if p not in counter:
+                    if (step, p.device) not in to:
+                        to[step, p.device] = torch.zeros(1, dtype=torch.int64, device=p.device)
+                    counter[p] = to[step, p.device]
                 have = self.state.get(p)
                 if have is not None and (self._order.get(p) != _layout(p)
                                          or have["exp_avg"].device != p.device):
                     have = None
-                new[p] = s = dict(step=step)
+                new[p] = s = dict(step=counter[p])
                 for name, t in moments.items():
                     s[name] = have[name] if have is not None else \
                         torch.empty_like(p, dtype=t.dtype) if self.state_bits == 32 else \

@@ -267,3 +267,74 @@ def test_a_state_of_torchs(lib):
         assert int(opt.state[p]["step"]) == 1
     with pytest.raises(ValueError):
         AdamW([p]).load_state_dict(torch.optim.Adam([p], weight_decay=0.1).state_dict())
+
+
+def counters(opt, ps):
+    return [opt.state[p]["step"].data_ptr() for p in ps]
+
+
+def test_a_counter_for_each_history(lib, monkeypatch):
+    """t is a parameter's own: those whose gradients came in the same steps share a counter (one
+    launch before the updates), a parameter that comes later or stays out has its own from there."""
+    from gnnea.optim import AdamW
+    ps = parameters((3,), (4,), (5,), (6,))
+    ps[3].grad = None
+    opt = AdamW(ps)
+    opt.step()
+    assert len(set(counters(opt, ps[:3]))) == 1 and lib.count("gnnea_adamw_begin") == 1
+    first = counters(opt, ps[:1])[0]
+    ps[3].grad = torch.ones(6)
+    opt.step()  # the newcomer counts from 0
+    assert counters(opt, ps[:3]) == [first] * 3 and counters(opt, ps)[3] != first
+    assert lib.count("gnnea_adamw_begin") == 1 + 2
+    ps[1].grad = None
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    before = len(lib.names)
+    with pytest.raises(RuntimeError):  # a graph would set the counter back at every replay
+        opt.step()
+    assert len(lib.names) == before and counters(opt, ps[:3]) == [first] * 3
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    opt.state[ps[0]]["step"].fill_(7)
+    opt.step()  # the one that stays out keeps the old count, in a counter of its own
+    assert counters(opt, [ps[0], ps[2]]) == [first] * 2 and counters(opt, ps)[1] != first
+    assert int(opt.state[ps[1]]["step"]) == 7
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    opt.step()  # the same parameters as in the step before: nothing to part
+
+
+def test_steps_that_differ_are_loaded(lib):
+    """A state whose parameters have taken different numbers of steps keeps each; counters that are
+    there are written into."""
+    from gnnea.optim import AdamW
+    ps = parameters((3,), (4,), (5,))
+    other = torch.optim.AdamW(ps)
+    other.step()
+    sd = other.state_dict()
+    for i, t in enumerate((1000, 1, 1000)):
+        sd["state"][i]["step"] = torch.tensor(float(t))
+    opt = AdamW(ps)
+    opt.load_state_dict(sd)
+    assert [int(opt.state[p]["step"]) for p in ps] == [1000, 1, 1000]
+    assert len(set(counters(opt, ps))) == 2
+    was = counters(opt, ps)
+    sd["state"][1]["step"] = torch.tensor(5.0)
+    opt.load_state_dict(sd)
+    assert counters(opt, ps) == was and [int(opt.state[p]["step"]) for p in ps] == [1000, 5, 1000]
+    sd["state"][2]["step"] = torch.tensor(2.0)
+    opt.load_state_dict(sd)
+    assert [int(opt.state[p]["step"]) for p in ps] == [1000, 5, 2]
+    opt.load_state_dict(opt.state_dict())
+    assert [int(opt.state[p]["step"]) for p in ps] == [1000, 5, 2]
+    lib.names.clear()
+    opt.step()
+    assert lib.count("gnnea_adamw_begin") == 3
+
+
+def test_a_refused_step_leaves_no_state(lib):
+    """A later group's refusal comes before anything is made or parted for an earlier one."""
+    from gnnea.optim import AdamW
+    p, q, r = parameters((3,), (4,), (5,))
+    opt = AdamW([dict(params=[p, q]), dict(params=[r])])
+    r.data = torch.zeros(5).double()
+    refused(lib, opt, TypeError)
+    assert not opt.state
