@@ -223,10 +223,31 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamList L, const AdamHyper
       }
       mt = wave_max_u32(mt);
       ut = wave_max_u32(ut);
+      // An element whose moments are not finite is lost, as it is with 32 bits: NaN from here on
+      // (e4m3's code for it).  The block's exponents go by the others, which keep what they have.
+      uint32_t lost = 0;
+      if (max(mt, ut) >= 0x7f800000u) {
+        mt = ut = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a = __builtin_bit_cast(uint32_t, m[u][k]) & 0x7fffffffu;
+          const uint32_t b = __builtin_bit_cast(uint32_t, root[k]) & 0x7fffffffu;
+          if (max(a, b) >= 0x7f800000u) {
+            lost |= 0x7fu << (8 * k);
+            m[u][k] = __builtin_nanf("");
+          } else {
+            mt = max(mt, a);
+            ut = max(ut, b);
+          }
+        }
+        mt = wave_max_u32(mt);
+        ut = wave_max_u32(ut);
+      }
       // the smallest exponents under which all of m are below 448 = 1.75 2^8, and all of u below
-      // (1 + 15/16), so that neither rounds past its largest code; 1..254 for non-finite values
+      // (1 + 15/16), so that neither rounds past its largest code (e <= 247, f <= 192: a root of a
+      // finite v is below 2^64)
       const int e = max(1, (int)((mt + (1u << 21)) >> 23) - 8);
-      const int f = min(254, max(17, (int)((ut + (1u << 19)) >> 23)));
+      const int f = max(17, (int)((ut + (1u << 19)) >> 23));
       const float ms = pow2(254 - e), us = pow2(254 - f);
       int w = __builtin_amdgcn_cvt_pk_fp8_f32(m[u][0] * ms, m[u][1] * ms, 0, false);
       w = __builtin_amdgcn_cvt_pk_fp8_f32(m[u][2] * ms, m[u][3] * ms, w, true);
@@ -238,7 +259,7 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamList L, const AdamHyper
         const int q = (int)(__builtin_bit_cast(uint32_t, root[k] * us) - (112u << 23) + chance) >> 19;
         c |= (root[k] == 0.f ? 0u : (uint32_t)min(255, max(1, q))) << (8 * k);
       }
-      store4b<NT>((uint8_t*)t.m + at, left, (uint32_t)w);
+      store4b<NT>((uint8_t*)t.m + at, left, (uint32_t)w | lost);
       store4b<NT>((uint8_t*)t.v + at, left, c);
       if (lane == 0) {
         t.scales[b0 >> 8] = (uint8_t)e;

@@ -901,6 +901,8 @@ int gnnea_norm_bwd(const gnnea_norm* a, void* ws /* 16-B aligned */, int64_t ws_
  *   v: its root u, unsigned; code 0 is 0, else (1 + (c % 16) / 16) 2^(c / 16 - 15) times
  *      2^(scales[1][b] - 127); rounded up or down with the odds of its place between two codes,
  *      by a hash of (seed, t, tensor, element)
+ * An element whose moments are not finite is NaN from then on (m's code 0x7f; p), and has no part
+ * in its block's exponents.
  * The update uses the moments before they are rounded.  p and g have one type (GNNEA_F32 or
  * GNNEA_BF16) and any alignment; `tensors` is host memory, read before the call returns.
  *   gnnea_adamw_norm   sums of squares of the gradients, gnnea_adamw_norm_parts(...) doubles
