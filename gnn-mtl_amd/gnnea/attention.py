@@ -12,7 +12,7 @@ import torch
 from . import _lib
 from ._lib import AttnProblem, check, ptr, stream_of
 from .graph import csr_of
-from .ops import FEATURE_DTYPES, _ld, _rows
+from .ops import FEATURE_DTYPES, _ld, _rows, needs_node
 
 MAX_D_HEAD = 256
 # rows with more stored entries are cut into pieces of as many, one wave each
@@ -167,6 +167,6 @@ def dot_attention(adj, q, k, v, heads, kv_heads=None, scale=None):
     q, k, v = _rows(q), _rows(k), _rows(v)
     if _ld(k) != _ld(v):  # the kernels form one row offset for both
         k, v = k.contiguous(), v.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if needs_node(q, k, v):
         return DotAttentionFn.apply(q, k, v, csr, meta)
     return _forward(q, k, v, csr, meta, False)[0]

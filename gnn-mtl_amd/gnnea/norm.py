@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import NormProblem, check, ptr, stream_of
-from .ops import FEATURE_DTYPES, _ld, _rows
+from .ops import FEATURE_DTYPES, _ld, _rows, needs_node
 
 KINDS = {"rms": _lib.GNNEA_NORM_RMS, "layer": _lib.GNNEA_NORM_LAYER}
 MAX_D = 8192
@@ -180,8 +180,7 @@ def _kind(kind, eps):
 
 
 def _apply(x, y, gate, vecs, meta):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, y, gate) + tuple(vecs)):
+    if needs_node(x, y, gate, *vecs):
         return NormFn.apply(x, y, gate, *vecs, meta)
     return _forward(x, y, gate, vecs, meta, False)[:2]
 

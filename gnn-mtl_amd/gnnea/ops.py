@@ -9,6 +9,7 @@ import weakref
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, ptr, stream_of
@@ -46,6 +47,14 @@ def _f32c(t):
 
 
 FEATURE_DTYPES = (torch.float32, torch.bfloat16)
+
+
+def needs_node(*tensors):
+    """Whether a call on these tensors has to go through its autograd node: for a gradient, or,
+    inside a forward-mode level, to refuse a tangent (dual tensors do not require grad)."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _rows(t, dtype=None):
