@@ -182,13 +182,15 @@ extern "C" int gnnea_coo_to_csr(const void* row_idx, const void* col_idx, int in
 }
 
 namespace gnnea {
-// row id of every CSR entry (used to build the transpose from (col, row) pairs)
+// row id of every CSR entry (used to build the transpose from (col, row) pairs); a wave per row, and
+// over more rows in turn where there are so many that 64 work-items each would pass 2^32
+constexpr int kExpandBlocks = 1 << 23;
 __global__ void k_expand_rows(const int32_t* __restrict__ rowptr, int32_t n_rows,
                               int32_t* __restrict__ row_out) {
-  const int r = blockIdx.x * 4 + wave_id();
-  if (r >= n_rows) return;
-  const int beg = rowptr[r], end = rowptr[r + 1];
-  for (int e = beg + lane_id(); e < end; e += 64) row_out[e] = r;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + wave_id(); r < n_rows; r += (int64_t)gridDim.x * 4) {
+    const int beg = rowptr[r], end = rowptr[r + 1];
+    for (int e = beg + lane_id(); e < end; e += 64) row_out[e] = (int32_t)r;
+  }
 }
 }  // namespace gnnea
 
@@ -197,7 +199,9 @@ extern "C" int gnnea_csr_expand_rows(const int32_t* rowptr, int32_t n_rows, int6
   if (n_rows < 0 || nnz < 0) return GNNEA_EINVAL;
   if (n_rows == 0 || nnz == 0) return 0;
   if (!rowptr || !row_out) return GNNEA_EINVAL;
-  hipLaunchKernelGGL(gnnea::k_expand_rows, dim3(gnnea::div_up(n_rows, 4)), dim3(256), 0,
+  const int blocks = gnnea::div_up(n_rows, 4);
+  hipLaunchKernelGGL(gnnea::k_expand_rows,
+                     dim3(blocks < gnnea::kExpandBlocks ? blocks : gnnea::kExpandBlocks), dim3(256), 0,
                      (hipStream_t)stream, rowptr, n_rows, row_out);
   GNNEA_LAUNCH_CHECK();
   return 0;
