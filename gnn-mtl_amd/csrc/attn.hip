@@ -43,9 +43,11 @@ constexpr float kLog2e = 1.44269504088896340736f;
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 // hs: log2 of the heads that a wave's groups take at once; share: query heads per key/value head,
-// ss: its log2 where it has one, else -1
+// ss: its log2 where it has one, else -1; row0, items: the launch's first row, and its pieces
 struct AttnPlan { int lph, nch, hs, share, ss, units_y; bool full; };
-struct AttnShape { int hs, share, ss; };
+struct AttnShape { int hs, share, ss, row0, items; };
+// Rows of one launch: 64 work-items each, which have to stay below 2^32 in all.
+constexpr int kAttnRows = 1 << 25;
 __device__ __forceinline__ int by_share(const AttnShape& p, int x) {
   return p.ss >= 0 ? x >> p.ss : (int)((uint32_t)x / (uint32_t)p.share);
 }
@@ -193,19 +195,20 @@ struct AttnUnit { int row, beg, end, slot; };
 // The wave's piece of a long row (their workgroups come first: they run longest), or its row (slot
 // < 0).  Consecutive rows share an XCD: neighbours in the ring of entities share keys, and rows
 // that are not whole cache lines share lines.  False: nothing to do.
-__device__ __forceinline__ bool attn_unit(const gnnea_attn& a, AttnUnit& u) {
-  const int pb = (a.n_items + 3) / 4, b = blockIdx.x;
+__device__ __forceinline__ bool attn_unit(const gnnea_attn& a, const AttnShape& S, AttnUnit& u) {
+  const int pb = (S.items + 3) / 4, b = blockIdx.x;
   if (b < pb) {
     const int id = b * 4 + wave_id();
-    if (id >= a.n_items) return false;
+    if (id >= S.items) return false;
     const int4 it = ((const int4*)a.items)[id];
     u.row = it.x; u.beg = it.y; u.end = it.z; u.slot = it.w;
     return true;
   }
-  const int id = xcd_remap(b - pb, (int)gridDim.x - pb) * 4 + wave_id();
-  if (id >= a.n_rows) return false;
-  u.row = id; u.beg = a.rowptr[id]; u.end = a.rowptr[id + 1]; u.slot = -1;
-  return a.limit == 0 || u.end - u.beg <= a.limit;
+  const uint32_t at = (uint32_t)xcd_remap(b - pb, (int)gridDim.x - pb) * 4 + wave_id();
+  const uint32_t id = (uint32_t)S.row0 + at;
+  if (id >= (uint32_t)a.n_rows) return false;
+  u.row = (int)id; u.beg = a.rowptr[id]; u.end = a.rowptr[id + 1]; u.slot = -1;
+  return a.n_items == 0 || u.end - u.beg <= a.limit;
 }
 
 // Entries that a group loads before it computes any.  More in flight per wave cost registers, and
@@ -259,7 +262,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd(const gnnea_attn a, const Attn
                                                   float* __restrict__ ws) {
   constexpr int V = RowChunk<T>::V, G = 64 / LPH, U = Steps<NCH>::U;
   AttnUnit u;
-  if (!attn_unit(a, u)) return;
+  if (!attn_unit(a, S, u)) return;
   const int lane = lane_id(), grp = lane / LPH, dh = a.d_head;
   const Lane<T, LPH, NCH, FULL> L{dh, lane % LPH};
   const int head = (blockIdx.y << S.hs) + (grp & ((1 << S.hs) - 1)), slot = grp >> S.hs, eps = G >> S.hs;
@@ -363,7 +366,7 @@ __global__ __launch_bounds__(256) void k_attn_rows(const gnnea_attn a, const Att
                                                    float* __restrict__ ws) {
   constexpr int V = RowChunk<T>::V, G = 64 / LPH, U = Steps<NCH>::U;
   AttnUnit u;
-  if (!attn_unit(a, u)) return;
+  if (!attn_unit(a, S, u)) return;
   const int lane = lane_id(), grp = lane / LPH, dh = a.d_head;
   const Lane<T, LPH, NCH, FULL> L{dh, lane % LPH};
   const int head = (blockIdx.y << S.hs) + (grp & ((1 << S.hs) - 1)), slot = grp >> S.hs, eps = G >> S.hs;
@@ -488,7 +491,7 @@ __global__ __launch_bounds__(256) void k_attn_cols(const gnnea_attn a, const Att
                                                    float* __restrict__ ws) {
   constexpr int V = RowChunk<T>::V, G = 64 / LPH, U = Steps<NCH>::U;
   AttnUnit u;
-  if (!attn_unit(a, u)) return;
+  if (!attn_unit(a, S, u)) return;
   const int lane = lane_id(), grp = lane / LPH, dh = a.d_head;
   const Lane<T, LPH, NCH, FULL> L{dh, lane % LPH};
   const int kvh = (blockIdx.y << S.hs) + (grp & ((1 << S.hs) - 1)), slot = grp >> S.hs, pps = G >> S.hs;
@@ -716,14 +719,17 @@ static AttnPlan attn_plan(const gnnea_attn* a, int pass) {
 template <typename T, int LPH, int NCH, bool FULL>
 static void attn_launch(const gnnea_attn& a, int pass, const AttnPlan& p, float* ws,
                         hipStream_t s) {
-  const dim3 grid(div_up(a.n_items, 4) + div_up(a.n_rows, 4), p.units_y);
-  const AttnShape sh = {p.hs, p.share, p.ss};
-  if (pass == GNNEA_ATTN_FWD)
-    hipLaunchKernelGGL((k_attn_fwd<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, sh, ws);
-  else if (pass == GNNEA_ATTN_BWD_ROWS)
-    hipLaunchKernelGGL((k_attn_rows<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, sh, ws);
-  else
-    hipLaunchKernelGGL((k_attn_cols<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, sh, ws);
+  for (int64_t row0 = 0; row0 < a.n_rows; row0 += kAttnRows) {
+    const int64_t rows = a.n_rows - row0 < kAttnRows ? a.n_rows - row0 : kAttnRows;
+    const AttnShape sh = {p.hs, p.share, p.ss, (int)row0, row0 ? 0 : a.n_items};
+    const dim3 grid((unsigned)((sh.items + 3ll) / 4 + (rows + 3) / 4), p.units_y);
+    if (pass == GNNEA_ATTN_FWD)
+      hipLaunchKernelGGL((k_attn_fwd<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, sh, ws);
+    else if (pass == GNNEA_ATTN_BWD_ROWS)
+      hipLaunchKernelGGL((k_attn_rows<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, sh, ws);
+    else
+      hipLaunchKernelGGL((k_attn_cols<T, LPH, NCH, FULL>), grid, dim3(256), 0, s, a, sh, ws);
+  }
 }
 template <typename T, int LPH, int NCH>
 static void attn_launch(const gnnea_attn& a, int pass, const AttnPlan& p, float* ws,

@@ -953,7 +953,7 @@ int gnnea_adamw_moments(const gnnea_adamw_tensor* tensors, int32_t count, void* 
  *   _bwd_cols  dk, dv (summed over the heads that share a key/value head) over the transposed
  *              matrix's rows; reads stat
  * Rows of dq, dk, dv without entries are written with zeros.  Sums are fp32 in a fixed order.
- * Rows of more than `limit` entries (0: none) are left to pieces: items {row, begin, end, slot}
+ * Where there are pieces (n_items > 0), rows of more than `limit` entries are left to them: items {row, begin, end, slot}
  * (int32 x 4; slots 0 .. n_items - 1) and, joined in order, long_rows with their slots
  * long_ptr[w] .. long_ptr[w + 1] - 1.  They depend on rowptr alone (built once per matrix).
  * ------------------------------------------------------------------------------------------ */
