@@ -208,6 +208,8 @@ def residual_norm(x, y, gate=None, scale=None, post_weight=None, post_bias=None,
     if scale is not None and not isinstance(scale, torch.Tensor):
         alpha, scale = float(scale), None
     elif scale is not None and scale.numel() == 1:
+        if scale.dtype == torch.bfloat16:  # its gradient, a sum over columns, is then rounded once
+            scale = scale.float()
         scale = scale.reshape(1).expand(x.shape[1])
     y = _matrix("y", y, x)
     names = ("scale", "post_weight", "post_bias", "pre_weight", "pre_bias", "gate")
