@@ -17,6 +17,8 @@ BLOCK = _lib.GNNEA_ADAMW_BLOCK
 
 def _dense(t):
     """Whether t's elements fill memory without gaps, in whatever order of dimensions."""
+    if t.numel() == 0:
+        return True
     need = 1
     for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
         if stride != need:

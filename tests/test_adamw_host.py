@@ -338,3 +338,16 @@ def test_a_refused_step_leaves_no_state(lib):
     r.data = torch.zeros(5).double()
     refused(lib, opt, TypeError)
     assert not opt.state
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("shape", [(0,), (0, 4), (5, 0), (2, 0, 3)])
+def test_parameters_without_elements(lib, shape, bits):
+    """Dense whatever their strides; a step, its state and loading it leave the others theirs."""
+    from gnnea.optim import AdamW
+    p, q = parameters(shape, (3,))
+    opt = AdamW([p, q], state_bits=bits)
+    opt.step()
+    opt.load_state_dict(opt.state_dict())
+    opt.step()
+    assert opt.state[p]["exp_avg"].numel() == 0 and lib.count("gnnea_adamw_step") == 2
