@@ -54,7 +54,11 @@ def needs_node(*tensors):
     inside a forward-mode level, to refuse a tangent (dual tensors do not require grad)."""
     if getattr(forward_ad, "_current_level", 0) >= 0:
         return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _rows(t, dtype=None):

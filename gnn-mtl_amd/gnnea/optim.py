@@ -5,14 +5,17 @@ the same loop (``weight_decay=0`` is Adam), with the gradients' global norm clip
 step where ``max_norm`` is given.  The step counter and the learning rate stay on the device, so a
 step can be captured into a HIP graph as it is.
 """
-import numpy as np
+from array import array
+
 import torch
 
 from . import _lib
-from ._lib import check, ptr, stream_of
+from ._lib import check, stream_of
 from .ops import FEATURE_DTYPES
 
 BLOCK = _lib.GNNEA_ADAMW_BLOCK
+DESCRIPTOR = len(_lib.AdamwTensor._fields_)  # its 64-bit words
+CTL = _lib.GNNEA_ADAMW_CTL_BYTES // 4
 
 
 def _dense(t):
@@ -67,6 +70,9 @@ class AdamW(torch.optim.Optimizer):
         self.seed = int(seed) & 0xffffffff
         self.grad_norm = None
         self._order = {}  # the layout that a parameter's moments have
+        # of the states that have been compared with their parameter: their tensors, and what the
+        # parameter was then (shape, strides, device, length)
+        self._known = {}
         self._base = []  # number of a group's first parameter in the hash of the 8-bit rounding
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
@@ -90,17 +96,21 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("gnnea.AdamW: lr must not be negative (got %r)" % (lr,))
 
     @classmethod
-    def _check_group(cls, group):
+    def _check_numbers(cls, group):
         cls._check_lr(group["lr"])
-        eps, weight_decay, betas = group["eps"], group["weight_decay"], group["betas"]
-        if not eps > 0 or not weight_decay >= 0:
+        betas = group["betas"]
+        if not group["eps"] > 0 or not group["weight_decay"] >= 0:
             raise ValueError("gnnea.AdamW: eps must be positive and weight_decay not negative")
-        if len(betas) != 2 or not all(0 <= b < 1 for b in betas):
+        if len(betas) != 2 or not 0 <= betas[0] < 1 or not 0 <= betas[1] < 1:
             raise ValueError("gnnea.AdamW: betas must be in [0, 1) (got %r)" % (betas,))
+
+    @classmethod
+    def _check_group(cls, group):
+        cls._check_numbers(group)
         for name in ("amsgrad", "maximize", "differentiable"):
             if group.get(name):
                 raise ValueError("gnnea.AdamW: %s is not done here" % name)
-        if weight_decay and not group.get("decoupled_weight_decay", True):
+        if group["weight_decay"] and not group.get("decoupled_weight_decay", True):
             raise ValueError("gnnea.AdamW: weight_decay here is decoupled from the gradient")
         if len(set(map(id, group["params"]))) != len(group["params"]):
             raise ValueError("gnnea.AdamW: a parameter is in its group twice")
@@ -113,7 +123,7 @@ class AdamW(torch.optim.Optimizer):
     def __getstate__(self):
         return dict(super().__getstate__(), state_bits=self.state_bits, max_norm=self.max_norm,
                     seed=self.seed, grad_norm=None, _base=self._base,
-                    _order=self._order)
+                    _order=self._order, _known={})
 
     def _init_state(self, p, step):
         s = self.state[p]
@@ -130,32 +140,50 @@ class AdamW(torch.optim.Optimizer):
             s["scales"] = torch.full((2, -(-n // BLOCK)), 127, dtype=torch.uint8, device=p.device)
         return s
 
+    def _names(self):
+        return ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_rms",
+                                                                      "scales")
+
+    def _state_row(self, p, s, shape, stride, device):
+        """m, the second moment, the scales and the length of a state, for a descriptor, after p, of
+        this shape, strides and device, and its state have been compared."""
+        k = self._known.get(id(s))
+        if self.state_bits == 32:
+            m, v, scales = s["exp_avg"], s["exp_avg_sq"], None
+        else:
+            m, v, scales = s["exp_avg"], s["exp_avg_rms"], s["scales"]
+        if k is None or k[0] is not m or k[1] is not v or k[2] is not scales or k[3] != shape or \
+                k[4] != stride or k[5] != device:
+            self._check_state(p, s)
+            k = self._known[id(s)] = (m, v, scales, shape, stride, device, p.numel())
+        return m.data_ptr(), v.data_ptr(), 0 if scales is None else scales.data_ptr(), k[6]
+
     def _check_state(self, p, s):
-        if s["exp_avg"].device != p.device:
-            raise ValueError("gnnea.AdamW: a parameter was moved to %s, its state is on %s"
-                             % (p.device, s["exp_avg"].device))
-        order = self._order.get(p)
-        if order is None:
-            self._order[p] = _layout(p)
-        elif (order[0] != p.shape or order[1] != p.stride()) and order != _layout(p):
+        order = self._order.setdefault(p, _layout(p))
+        if order != _layout(p):
             raise ValueError("gnnea.AdamW: a parameter's shape and strides were %s at its first step "
                              "and are %s now" % (order, _layout(p)))
-
-    def _state_row(self, s):
-        """m, the second moment, the scales and the length of a state, for a descriptor."""
-        m = s["exp_avg"]
-        if self.state_bits == 32:
-            return (m.data_ptr(), s["exp_avg_sq"].data_ptr(), 0, m.numel())
-        return (m.data_ptr(), s["exp_avg_rms"].data_ptr(), s["scales"].data_ptr(), m.numel())
+        n = p.numel()
+        for name in self._names():
+            t = s[name]
+            if t.device != p.device:
+                raise ValueError("gnnea.AdamW: a parameter is on %s, its state on %s"
+                                 % (p.device, t.device))
+            if self.state_bits == 32:
+                ok = t.dtype == torch.float32 and _layout(t) == order
+            else:
+                ok = t.dtype == torch.uint8 and t.is_contiguous() and tuple(t.shape) == (
+                    (2, -(-n // BLOCK)) if name == "scales" else (n,))
+            if not ok:
+                raise ValueError("gnnea.AdamW: a state's %s is not one of its parameter (%s %s)"
+                                 % (name, t.dtype, tuple(t.shape)))
 
     @staticmethod
     def _gradient(p, g, n):
         """g with p's order of elements.  (torch compares the two where a gradient is assigned; the
         parameter's data, type or place may have been replaced since.)"""
-        if p.dtype not in FEATURE_DTYPES:
-            raise TypeError("gnnea.AdamW: fp32 or bf16 parameters required (got %s)" % p.dtype)
-        if g.is_sparse or g.dtype != p.dtype or g.shape != p.shape or g.device != p.device or \
-                p.numel() != n:
+        if g.layout is not torch.strided or g.dtype != p.dtype or g.shape != p.shape or \
+                g.device != p.device or p.numel() != n:
             raise ValueError("gnnea.AdamW: gradients must be dense and like their parameter")
         if p.is_contiguous():
             return g if g.is_contiguous() else g.contiguous()
@@ -175,16 +203,17 @@ class AdamW(torch.optim.Optimizer):
         todo, held, device = [], [], None
         state = self.state
         for base, group in zip(self._base, self.param_groups):
-            # by counter: [counter, rows by type, states without a gradient]; the parameters'
-            # first steps under None
-            counters = {}
+            # by counter: the counter, descriptors by type, states without a gradient; under None the
+            # parameters (with gradient and index) that take their first step
+            counters, c = {}, None
             for i, p in enumerate(group["params"]):
                 s, g = state.get(p), p.grad
                 if s is not None:
                     step = s["step"]
-                    c = counters.get(id(step))
-                    if c is None:
-                        c = counters[id(step)] = (step, {}, [])
+                    if c is None or c[0] is not step:
+                        c = counters.get(id(step))
+                        if c is None:
+                            c = counters[id(step)] = (step, {}, [])
                     if g is None:
                         c[2].append(s)
                 if g is None:
@@ -198,20 +227,29 @@ class AdamW(torch.optim.Optimizer):
                     c = counters.get(None)
                     if c is None:
                         c = counters[None] = (None, {}, [])
+                dtype = p.dtype
+                rows = c[1].get(dtype)
+                if rows is None:
+                    if dtype not in FEATURE_DTYPES:
+                        raise TypeError("gnnea.AdamW: fp32 or bf16 parameters required (got %s)"
+                                        % dtype)
+                    rows = c[1][dtype] = []
+                if s is None:
                     g = self._gradient(p, g, p.numel())
-                    c[1].setdefault(p.dtype, []).append((p, g, base + i))
+                    rows.append((p, g, base + i))
                 else:
-                    self._check_state(p, s)
-                    row = self._state_row(s)
-                    g = self._gradient(p, g, row[3])
-                    c[1].setdefault(p.dtype, []).append((p.data_ptr(), g.data_ptr()) + row
-                                                        + (base + i,))
+                    shape, stride = p.shape, p.stride()
+                    m, v, scales, n = self._state_row(p, s, shape, stride, device)
+                    if g.is_sparse or g.dtype is not dtype or g.shape != shape or \
+                            g.stride() != stride or g.device != device:
+                        g = self._gradient(p, g, n)
+                    rows += (p.data_ptr(), g.data_ptr(), m, v, scales, n, base + i)
                 held.append(g)
             counters = [c for c in counters.values() if c[1]]
             if not counters:
                 continue
-            lr = group["lr"]  # may have been replaced since the group was checked
-            self._check_lr(lr)
+            self._check_numbers(group)  # they may have been replaced since the group was made
+            lr = group["lr"]
             if isinstance(lr, torch.Tensor) and lr.device != device:
                 raise ValueError("gnnea.AdamW: lr is on %s, the parameters on %s"
                                  % (lr.device, device))
@@ -231,14 +269,15 @@ class AdamW(torch.optim.Optimizer):
                 if step is None:
                     step = torch.zeros(1, dtype=torch.int64, device=device)
                     for rows in lists.values():
-                        rows[:] = [(p.data_ptr(), g.data_ptr())
-                                   + self._state_row(self._init_state(p, step)) + (index,)
-                                   for p, g, index in rows]
+                        rows[:] = [x for p, g, index in rows for x in (
+                            p.data_ptr(), g.data_ptr(),
+                            *self._state_row(p, self._init_state(p, step), p.shape, p.stride(),
+                                             device), index)]
                 arrays = []
                 for dtype, rows in lists.items():
-                    table = np.array(rows, dtype=np.int64)
+                    table = array("q", rows)
                     held.append(table)
-                    arrays.append((table.ctypes.data, len(rows), _lib.GNNEA_BF16
+                    arrays.append((table.buffer_info()[0], len(table) // DESCRIPTOR, _lib.GNNEA_BF16
                                    if dtype == torch.bfloat16 else _lib.GNNEA_F32))
                 groups.append((group, step, arrays))
         if not groups:
@@ -246,31 +285,31 @@ class AdamW(torch.optim.Optimizer):
         L = _lib.lib()
         with _lib.on_device(device):
             stream = stream_of(device)
-            parts, n_parts = None, 0
+            n_parts, counts = 0, ()
             if self.max_norm is not None:
                 counts = [[int(L.gnnea_adamw_norm_parts(a, c)) for a, c, _ in arrays]
                           for _, _, arrays in groups]
                 n_parts = sum(map(sum, counts))
-                parts = torch.empty(max(n_parts, 1), dtype=torch.float64, device=device)
-                at = parts.data_ptr()
-                for (_, _, arrays), of in zip(groups, counts):
-                    for (a, c, code), m in zip(arrays, of):
-                        check(L.gnnea_adamw_norm(a, c, code, at, m, stream))
-                        at += 8 * m
+            # the norm's parts (8 bytes each), then the scalars of each update
+            scratch = torch.empty(2 * n_parts + len(groups) * CTL, dtype=torch.float32, device=device)
+            parts = at = scratch.data_ptr()
+            for (_, _, arrays), of in zip(groups, counts):
+                for (a, c, code), m in zip(arrays, of):
+                    check(L.gnnea_adamw_norm(a, c, code, at, m, stream))
+                    at += 8 * m
             for group, step, arrays in groups:
                 lr, (b1, b2) = group["lr"], group["betas"]
                 on_device = isinstance(lr, torch.Tensor)
-                ctl = torch.empty(_lib.GNNEA_ADAMW_CTL_BYTES // 4, dtype=torch.float32,
-                                  device=device)
-                check(L.gnnea_adamw_begin(ptr(parts), n_parts, self.max_norm or 0.0, b1, b2,
-                                          0.0 if on_device else lr,
-                                          ptr(lr) if on_device else None, self.seed, ptr(step),
-                                          ptr(ctl), stream))
+                check(L.gnnea_adamw_begin(parts if n_parts else None, n_parts, self.max_norm or 0.0,
+                                          b1, b2, 0.0 if on_device else lr,
+                                          lr.data_ptr() if on_device else None, self.seed,
+                                          step.data_ptr(), at, stream))
                 for a, c, code in arrays:
                     check(L.gnnea_adamw_step(a, c, code, self.state_bits, b1, b2, group["eps"],
-                                             group["weight_decay"], ptr(ctl), stream))
-                if self.max_norm is not None:
-                    self.grad_norm = ctl[4]
+                                             group["weight_decay"], at, stream))
+                at += 4 * CTL
+            if self.max_norm is not None:
+                self.grad_norm = scratch[2 * n_parts + 4]
         return loss
 
     @torch.no_grad()
@@ -287,17 +326,17 @@ class AdamW(torch.optim.Optimizer):
                 elif self.state_bits == 32:
                     out.append((s["exp_avg"], s["exp_avg_sq"]))
                 else:
-                    self._check_state(p, s)
+                    row = self._state_row(p, s, p.shape, p.stride(), p.device)
                     m = torch.empty_like(p, dtype=torch.bfloat16)
-                    u = torch.empty_like(p, dtype=torch.bfloat16)
-                    rows.append((m.data_ptr(), u.data_ptr()) + self._state_row(s) + (0,))
+                    u = torch.empty_like(m)
+                    rows += (m.data_ptr(), u.data_ptr(), *row, 0)
                     out.append((m, u))
         if rows:
             device = next(m.device for m, _ in out if m is not None)
-            table = np.array(rows, dtype=np.int64)
+            table = array("q", rows)
             with _lib.on_device(device):
-                check(_lib.lib().gnnea_adamw_moments(table.ctypes.data, len(rows),
-                                                     stream_of(device)))
+                check(_lib.lib().gnnea_adamw_moments(table.buffer_info()[0],
+                                                     len(table) // DESCRIPTOR, stream_of(device)))
         return out
 
     def state_dict(self):
@@ -396,4 +435,4 @@ class AdamW(torch.optim.Optimizer):
             group.update(options)
         self.state.clear()
         self.state.update(new)
-        self._order = {p: _layout(p) for p in new}
+        self._order, self._known = {p: _layout(p) for p in new}, {}

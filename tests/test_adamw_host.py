@@ -351,3 +351,34 @@ def test_parameters_without_elements(lib, shape, bits):
     opt.load_state_dict(opt.state_dict())
     opt.step()
     assert opt.state[p]["exp_avg"].numel() == 0 and lib.count("gnnea_adamw_step") == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_that_was_replaced(lib, bits):
+    """Tensors put into the state by hand are held to its parameter's size, type, order and place."""
+    from gnnea.optim import AdamW
+    p, = parameters((40, 30))
+    opt = AdamW([p], state_bits=bits)
+    opt.step()
+    s = opt.state[p]
+    for name in opt._names():
+        was = s[name]
+        bad = [was.double(), was.flatten()[:-1], was.to("meta")]
+        bad += [transposed(was)] if was.dim() == 2 and was.shape[0] > 1 else []
+        for t in bad:
+            s[name] = t
+            refused(lib, opt)
+        s[name] = was.clone()
+        opt.step()
+
+
+@pytest.mark.parametrize("name,value", [("betas", (0.9, 1.0)), ("betas", (-0.1, 0.9)), ("eps", 0.0),
+                                        ("weight_decay", -1.0), ("eps", float("nan"))])
+def test_numbers_that_were_replaced(lib, name, value):
+    """Set after the group was made: refused before the first group's update."""
+    from gnnea.optim import AdamW
+    p, q = parameters((3,), (4,))
+    opt = AdamW([dict(params=[p]), dict(params=[q])], max_norm=1.0)
+    opt.step()
+    opt.param_groups[1][name] = value
+    refused(lib, opt)
