@@ -34,6 +34,8 @@ struct AdamList {
 struct AdamCtl { float coef, bc1, bc2, lr, norm; uint32_t key, skip, pad; };
 static_assert(sizeof(AdamCtl) == GNNEA_ADAMW_CTL_BYTES, "ctl");
 
+// the 32-bit finaliser of MurmurHash3 (A. Appleby), a bijection whose every input bit reaches every
+// output bit
 __device__ __forceinline__ uint32_t mix32(uint32_t h) {
   h = (h ^ (h >> 16)) * 0x85ebca6bu;
   h = (h ^ (h >> 13)) * 0xc2b2ae35u;
