@@ -147,16 +147,20 @@ class AdamW(torch.optim.Optimizer):
     def _state_row(self, p, s, shape, stride, device):
         """m, the second moment, the scales and the length of a state, for a descriptor, after p, of
         this shape, strides and device, and its state have been compared."""
-        k = self._known.get(id(s))
         if self.state_bits == 32:
-            m, v, scales = s["exp_avg"], s["exp_avg_sq"], None
+            m, v, scales, at = s["exp_avg"], s["exp_avg_sq"], None, 0
         else:
             m, v, scales = s["exp_avg"], s["exp_avg_rms"], s["scales"]
-        if k is None or k[0] is not m or k[1] is not v or k[2] is not scales or k[3] != shape or \
-                k[4] != stride or k[5] != device:
-            self._check_state(p, s)
-            k = self._known[id(s)] = (m, v, scales, shape, stride, device, p.numel())
-        return m.data_ptr(), v.data_ptr(), 0 if scales is None else scales.data_ptr(), k[6]
+            at = scales.data_ptr()
+        known = self._known.get(id(s))
+        if known is not None:
+            m0, v0, scales0, shape0, stride0, device0, n = known
+            if m is m0 and v is v0 and scales is scales0 and shape == shape0 and \
+                    stride == stride0 and device == device0:
+                return m.data_ptr(), v.data_ptr(), at, n
+        self._check_state(p, s)
+        self._known[id(s)] = m, v, scales, shape, stride, device, p.numel()
+        return m.data_ptr(), v.data_ptr(), at, p.numel()
 
     def _check_state(self, p, s):
         order = self._order.setdefault(p, _layout(p))
