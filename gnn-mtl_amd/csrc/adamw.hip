@@ -3,10 +3,13 @@
 // tensors of a list.  Moments in fp32, or in 8 bits with one exponent per 256 elements.
 //
 // Bytes per element: fp32 p, m, v read and written and g read, 28; with 8-bit moments 12 + 4 = 16
-// (+ 2/256 of scales); the norm reads g once more.  All three are bound by HBM: 300M elements take
-// 1.39 ms with 32-bit moments and 0.81 with 8 (6.0 and 5.9 TB/s; a plain copy of 4 GiB reaches
-// 4.7 here), reading out what the codes stand for 0.35 (1.8 GB).  A list of 12 tensors (0.54M
-// elements, clipped) is three launches of 7, 4 and 7 us.
+// (+ 2/256 of scales); the norm reads g once more.  With 32-bit moments that is what bounds it: 300M
+// elements take 1.39 ms (6.0 TB/s; a plain copy of 4 GiB reaches 4.7 here).  With 8 bits the update
+// also issues 81 vector instructions per element and lane (the hash, three fp64 operations, codes from
+// and to bytes), 0.62 ms of 300M elements' 0.82 to 0.90 (by machine; 5.3 to 5.9 TB/s), and most of
+// 8.4M bf16 elements' 29 us, whose 84 MB stay in the cache.  Reading out what the codes stand for
+// takes 0.36 ms (1.8 GB).  A list of 12 tensors (0.54M elements, clipped) is three launches of 7, 4
+// and 6 us.
 //
 // 8-bit moments.  m is e4m3 times a power of two per block (dequantising, scaling and finding the
 // largest value are exact, so a code depends on nothing but the value).  The second moment is
@@ -358,7 +361,7 @@ __global__ __launch_bounds__(256) void k_adamw_moments(const AdamList L) {
 
 // Lists that move more than the Infinity Cache holds are read and written past the caches: nothing
 // of them is there at the next step.  300M fp32 elements: 1552 -> 1393 us (6.0 TB/s) with 32-bit
-// moments, 906 -> 807 with 8; 8.6M bf16 elements (84 MB), which stay in the cache: 30 against 33 us.
+// moments, 906 -> 807 with 8 (one machine); 8.6M bf16 elements (84 MB), which stay in the cache: 30 against 33 us.
 constexpr int64_t kCacheBytes = 256 << 20;
 
 template <typename T, int BITS, bool NT>

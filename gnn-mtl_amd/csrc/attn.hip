@@ -26,10 +26,11 @@
 // The passes gather k and v (q and do) per entry.  Where a head is read by itself the cache that
 // holds the tables bounds them: 9.5M entries, 4 heads of 64 bf16, forward 1.23 ms (7.9 TB/s of
 // gathered bytes, as much as the aggregation kernels of this library reach); 290k entries, 4 heads
-// of 75 fp32: forward 93 us, row pass 105, column pass 119 (7.5, 6.6, 5.9 TB/s).  Where 4 query
-// heads share a key head, instructions do: 3.3M entries, 8 heads of 32 bf16 on 2: 212 us forward,
-// 289 rows (650 and 780 vector instructions a wave, 16 entries each), while the column pass,
-// which reads every query head, gathers again (460 us, 7.7 TB/s).
+// of 75 fp32: forward 93 us, row pass 108, column pass 120 (7.5, 6.4, 5.8 TB/s).  Where 4 query
+// heads share a key head, instructions do: 3.3M entries, 8 heads of 32 bf16 on 2: 211 us forward,
+// 313 rows (569 and 796 vector instructions a wave, 16 entries each: every query head has lanes of
+// its own, which load and unpack the shared key and value again), while the column pass, which reads
+// every query head, gathers again (460 us, 7.7 TB/s).
 //
 // One wave per row.  Rows of more than `limit` entries (hubs) are cut into pieces, one wave each,
 // whose partial sums a second launch joins in order; so no wave runs long after the others, and

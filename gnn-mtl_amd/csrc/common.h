@@ -220,8 +220,8 @@ template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float v) { return
 // ---- the x3 split (fp32 GEMMs on the bf16 matrix cores): x = h + m + l, each bf16, round to
 // nearest even: h = bf16(x), m = bf16(x - h), l = bf16(x - h - m).  Two elements at a time into
 // packed bf16 pairs (dword q of an 8-element MFMA operand holds elements 2q, 2q + 1): one
-// v_cvt_pk_bf16_f32 per level, the residuals as packed fp32 subtractions -- the same values as
-// element-wise casts with about half the vector instructions.
+// v_cvt_pk_bf16_f32 per level and pair -- the same values as element-wise casts.  (The residuals are
+// written as pairs too; packed fp32 instructions are off, so each takes two subtractions.)
 typedef float x3_f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 x3_bf16x2 __attribute__((ext_vector_type(2)));
 

@@ -943,9 +943,9 @@ int gnnea_adamw_moments(const gnnea_adamw_tensor* tensors, int32_t count, void* 
  *   o_i = sum_c p_ic v_c,   p_ic = softmax over the row's entries c of (scale q_i . k_c)
  * q, o: n_rows x heads d_head; k, v: n_cols x kv_heads d_head (type GNNEA_F32 or GNNEA_BF16, row
  * strides in elements, any alignment of an element); lse: n_rows x heads floats, the base-2
- * logarithm of the row's sum of exponentials; the row passes need ldk == ldv; a row without entries gives o = 0 and lse = -inf.  k and v of columns
- * that no row has stored are never read.  heads % kv_heads == 0, d_head <= 256.  The matrix's
- * values are not used.
+ * logarithm of the row's sum of exponentials; the row passes need ldk == ldv; a row without entries
+ * gives o = 0 and lse = -inf.  k and v of columns that no row has stored are never read.  heads %
+ * kv_heads == 0, d_head <= 256.  The matrix's values are not used.
  * Backward, the probabilities recomputed from the scores and lse, dp = do . v:
  *   _bwd_rows  dq_i = scale sum p (dp - delta) k, delta_i = sum p dp, over the matrix's rows (both
  *              sums about the dp of one of the row's entries: 0 exactly where all its dp are equal);
@@ -953,9 +953,10 @@ int gnnea_adamw_moments(const gnnea_adamw_tensor* tensors, int32_t count, void* 
  *   _bwd_cols  dk, dv (summed over the heads that share a key/value head) over the transposed
  *              matrix's rows; reads stat
  * Rows of dq, dk, dv without entries are written with zeros.  Sums are fp32 in a fixed order.
- * Where there are pieces (n_items > 0), rows of more than `limit` entries are left to them: items {row, begin, end, slot}
- * (int32 x 4; slots 0 .. n_items - 1) and, joined in order, long_rows with their slots
- * long_ptr[w] .. long_ptr[w + 1] - 1.  They depend on rowptr alone (built once per matrix).
+ * Where there are pieces (n_items > 0), rows of more than `limit` entries are left to them: items
+ * {row, begin, end, slot} (int32 x 4; slots 0 .. n_items - 1) and, joined in order, long_rows with
+ * their slots long_ptr[w] .. long_ptr[w + 1] - 1.  They depend on rowptr alone (built once per
+ * matrix); without them every row is one wave's.
  * ------------------------------------------------------------------------------------------ */
 typedef struct gnnea_attn {
   const int32_t *rowptr, *col;   /* the CSR; _bwd_cols: the transposed one */
