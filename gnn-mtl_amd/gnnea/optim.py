@@ -55,7 +55,8 @@ class AdamW(torch.optim.Optimizer):
                     the parameters as in torch.
     A parameter without a gradient is left as it is.  t counts a parameter's own steps, those with a
     gradient, as in torch; parameters of a group with the same history share one counter (and one
-    small launch per step).
+    small launch per step).  A captured step goes on with the counters it was captured with: capture
+    again after an eager step in which other parameters had gradients.
     Moments keep the order of memory that their parameter had when they were made: a parameter whose
     shape, strides or device is another after that is refused.  A state dict names the order of 8-bit
     codes ("layout"); without it they are taken as row-major."""
